@@ -1,0 +1,499 @@
+// Linear layers on dense weights of fewer bytes or of many experts: C[n][m] = sum_k B[n][k] * A[m][k], token-major as
+// the eleven-argument SpMM (third_party/ft.patch:2822-2846), with A and B
+//   - e4m3 codes with an fp32 scale per 128 x 128 block of A and per token and 128 features of B, or
+//   - fp16 / bf16,
+// and either one matrix A or one per group of consecutive tokens (experts; group borders are read on the device).
+//
+// A block takes 128 rows of A as the M side of tcgen05.mma and up to 128 tokens as its N side (N is a run-time field of
+// the instruction descriptor, so a group's last few tokens cost no more than they must), because weights are what there
+// is always plenty of: one token still fills the tensor core's 128 lanes and streams A at full rate.  A k-block is 128
+// bytes of K (64 halves or 128 codes, i.e. one scale block): one 128-byte-swizzled TMA box of A and one or a few of B
+// per ring stage, four MMAs.
+//
+// fp16 / bf16 accumulate the whole K range in TMEM.  With scales every k-block is a product of its own: the MMA warp
+// writes it to one of four TMEM buffers in turn, and the epilogue warps add it to fp32 registers, each column times
+// (token's scale) * (block's scale), while the tensor core is at the next ones.
+//
+// Roles: warp 0 TMA, warp 1 MMA issue and TMEM, warp 2 scales, warps 4..11 epilogue (warp % 4 = quarter of the TMEM
+// lanes, warp / 4 - 1 = every other chunk of columns).  Every wait is bounded; a block that gives up records it.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+
+#include "linear_plan.h"
+#include "ptx_sm100.cuh"
+
+namespace spmm_b200 {
+
+__device__ int g_linear_status;  // 1 after a bounded wait has given up
+
+constexpr int kLinearThreads   = 384;
+constexpr int kLinearMaxStages = 12;
+constexpr int kLinearMaxGroups = 1024;
+constexpr int kLinearRows      = 128;                // lanes of a block's tile
+constexpr int kLinearBoxBytes  = kLinearRows * 128;  // its operand, one k-block
+constexpr int kScaleSlots      = 8;
+constexpr int kEpilogueTeams   = 8;  // epilogue warps
+constexpr int kPieceCounters   = 4096;  // arrival counters at the head of a workspace
+constexpr int kLinearFixedSmem = 1024 /* alignment */ + 512 /* barriers */;
+
+struct LinearParams {
+    CUtensorMap  a_map, b_map;  // bytes: (K bytes, rows, groups)
+    const float* a_scales;      // [groups][ceil(M / 128)][kb]
+    const float* b_scales;      // [kb][N]
+    void*        C;
+    const int*   offsets;  // [groups + 1], or null: one group of all N tokens
+    unsigned*    counters;
+    float*       slots;
+    int          groups, m, n, kb;
+    int          nt;        // tokens per tile at most
+    int          b_box;     // tokens per TMA box
+    int          stages;
+    int          bf16;      // C (and 16-bit operands) are bf16, not fp16
+    int          overhead;  // see make_linear_partition
+};
+
+// Which part of the layer a tile is.
+struct LinearTile {
+    int group, m0, row0, rows;  // first row of A, first token, tokens
+};
+
+// One warp waits: lane 0 polls, the others follow.
+__device__ __forceinline__ bool linear_warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_word, int lane)
+{
+    int ok = 1;
+    if (lane == 0)
+        ok = ptx::mbar_wait_bounded(bar, parity, abort_word);
+    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+
+template<bool EIGHT>
+__global__ void __launch_bounds__(kLinearThreads, 1)
+linear_kernel(const __grid_constant__ LinearParams p)
+{
+    constexpr int NMAX = 128;             // columns of a TMEM buffer
+    constexpr int NBUF = 512 / NMAX;      // TMEM buffers
+    constexpr int CH   = 16;              // columns per chunk
+    constexpr int NCH  = NMAX / (2 * CH); // chunks per epilogue warp
+
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base   = (ptx::smem_addr(smem_raw) + 1023u) & ~1023u;
+    uint8_t*       smem        = smem_raw + (smem_base - ptx::smem_addr(smem_raw));
+    const uint32_t stage_bytes = kLinearBoxBytes + p.nt * 128u;
+    const uint32_t scale_off   = p.stages * stage_bytes;
+    const uint32_t bar_off     = scale_off + (EIGHT ? kScaleSlots * NMAX * 4u : 0u);
+    const uint32_t bar_base    = smem_base + bar_off;
+    float* const   scale_ring  = reinterpret_cast<float*>(smem + scale_off);
+    auto full       = [&](int s) { return bar_base + 8u * s; };
+    auto empty      = [&](int s) { return bar_base + 8u * (kLinearMaxStages + s); };
+    auto acc_full   = [&](int b) { return bar_base + 8u * (2 * kLinearMaxStages + b); };
+    auto acc_free   = [&](int b) { return bar_base + 8u * (2 * kLinearMaxStages + NBUF + b); };
+    auto scale_full = [&](int s) { return bar_base + 8u * (2 * kLinearMaxStages + 2 * NBUF + s); };
+    auto scale_free = [&](int s) { return bar_base + 8u * (2 * kLinearMaxStages + 2 * NBUF + kScaleSlots + s); };
+    constexpr uint32_t kWords = 8u * (2 * kLinearMaxStages + 2 * NBUF + 2 * kScaleSlots);
+    static_assert(kWords + 64 <= 512, "barrier block");
+    volatile uint32_t* tmem_slot  = reinterpret_cast<volatile uint32_t*>(smem + bar_off + kWords);
+    volatile int*      abort_word = reinterpret_cast<volatile int*>(smem + bar_off + kWords + 4);
+    int* const         warp_sums  = reinterpret_cast<int*>(smem + bar_off + kWords + 8);  // 12 words
+    int* const         tile_end   = reinterpret_cast<int*>(smem + bar_off + 512);         // per group, running total
+    int* const         group_row  = tile_end + p.groups;                                  // first token
+    int* const         group_rows = group_row + p.groups;                                 // tokens
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kLinearMaxStages; s++) {
+            ptx::mbar_init(full(s), 1);
+            ptx::mbar_init(empty(s), 1);
+        }
+        for (int b = 0; b < NBUF; b++) {
+            ptx::mbar_init(acc_full(b), 1);
+            ptx::mbar_init(acc_free(b), kEpilogueTeams);
+        }
+        for (int s = 0; s < kScaleSlots; s++) {
+            ptx::mbar_init(scale_full(s), 1);
+            ptx::mbar_init(scale_free(s), kEpilogueTeams);
+        }
+        *abort_word = 0;
+        ptx::mbar_init_fence();
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc(bar_base + kWords, 512);
+        ptx::tmem_relinquish();
+    }
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
+
+    // Tiles per group.  Borders are clamped to the tokens there are, so that a corrupt table cannot lead outside.
+    const int tiles_m = (p.m - 1) / kLinearRows + 1;
+    {
+        const int per = (p.groups + kLinearThreads - 1) / kLinearThreads;
+        const int e0  = min(static_cast<int>(threadIdx.x) * per, p.groups), e1 = min(e0 + per, p.groups);
+        int       sum = 0;
+        for (int e = e0; e < e1; e++) {
+            int from = 0, rows = p.n;
+            if (p.offsets) {
+                from = min(max(__ldg(p.offsets + e), 0), p.n);
+                rows = max(min(max(__ldg(p.offsets + e + 1), 0), p.n) - from, 0);
+            }
+            group_row[e]  = from;
+            group_rows[e] = rows;
+            sum += (rows + p.nt - 1) / p.nt * tiles_m;
+            tile_end[e] = sum;
+        }
+        int before = sum;  // becomes the total of the threads before this one
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, before, d);
+            if (lane >= d)
+                before += up;
+        }
+        if (lane == 31)
+            warp_sums[warp] = before;
+        before -= sum;
+        ptx::tc_fence_before_sync();
+        __syncthreads();
+        for (int w = 0; w < warp; w++)
+            before += warp_sums[w];
+        for (int e = e0; e < e1; e++)
+            tile_end[e] += before;
+        __syncthreads();
+        ptx::tc_fence_after_sync();
+    }
+    const uint32_t        tmem_base = *tmem_slot;
+    const LinearPartition part      = make_linear_partition(tile_end[p.groups - 1], p.kb, static_cast<int>(gridDim.x), p.overhead);
+    const int             worker    = static_cast<int>(blockIdx.x);
+
+    auto locate = [&](int tile) {
+        int lo = 0, hi = p.groups - 1;  // the first group whose running total is above `tile`
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (tile_end[mid] > tile)
+                hi = mid;
+            else
+                lo = mid + 1;
+        }
+        LinearTile t;
+        const int  rows = group_rows[lo], tiles_n = (rows + p.nt - 1) / p.nt;
+        const int  i    = tile - (lo > 0 ? tile_end[lo - 1] : 0);
+        t.group = lo;
+        t.m0    = i / tiles_n * kLinearRows;
+        t.row0  = i % tiles_n * p.nt;
+        t.rows  = min(p.nt, rows - t.row0);
+        t.row0 += group_row[lo];
+        return t;
+    };
+    auto columns = [&](const LinearTile& t) { return (t.rows + 15) & ~15; };
+
+    int issued = 0;  // ring stages filled (warp 0)
+    if (warp == 0) {
+        // ------------------------------------------------------------ TMA
+        if (lane == 0) {
+            bool ok = true;
+            int  s  = 0;
+            for (int i = 0; ok; i++) {
+                const LinearSegment seg = linear_segment(part, worker, i);
+                if (seg.tile < 0)
+                    break;
+                const LinearTile t     = locate(seg.tile);
+                const int        boxes = (columns(t) + p.b_box - 1) / p.b_box;
+                const uint32_t   bytes = kLinearBoxBytes + boxes * p.b_box * 128u;
+#pragma unroll 1
+                for (int k = seg.kb0; k < seg.kb1; k++) {
+                    if (issued >= p.stages) {
+                        ok = ptx::mbar_wait_bounded(empty(s), ((issued / p.stages) - 1) & 1, abort_word);
+                        if (!ok)
+                            break;
+                    }
+                    const uint32_t dst = smem_base + s * stage_bytes;
+                    ptx::mbar_arrive_expect_tx(full(s), bytes);
+                    ptx::tma_load_3d(dst, &p.a_map, k * 128, t.m0, t.group, full(s));
+                    for (int b = 0; b < boxes; b++)
+                        ptx::tma_load_3d(dst + kLinearBoxBytes + b * p.b_box * 128, &p.b_map, k * 128, t.row0 + b * p.b_box, 0, full(s));
+                    issued++;
+                    if (++s == p.stages)
+                        s = 0;
+                }
+            }
+        }
+    }
+    else if (warp == 1) {
+        // ------------------------------------------------------------ MMA
+        if (lane == 0) {
+            bool ok  = true;
+            int  use = 0, s = 0, phase = 0;  // use: TMEM buffers handed out
+            const uint64_t a_desc0 = ptx::make_smem_desc(smem_base, 16, 1024, ptx::kSwizzle128B);
+            for (int i = 0; ok; i++) {
+                const LinearSegment seg = linear_segment(part, worker, i);
+                if (seg.tile < 0)
+                    break;
+                const uint32_t idesc =
+                    ptx::make_idesc_f16_f32(kLinearRows, columns(locate(seg.tile)), false, false) | (!EIGHT && p.bf16 ? ptx::kIdescBf16 : 0u);
+#pragma unroll 1
+                for (int k = seg.kb0; k < seg.kb1; k++) {
+                    const uint32_t d_tmem = tmem_base + (use % NBUF) * NMAX;
+                    const bool     fresh  = EIGHT || k == seg.kb0;
+                    if (fresh && use >= NBUF && !ptx::mbar_wait_bounded(acc_free(use % NBUF), (use / NBUF - 1) & 1, abort_word)) {
+                        ok = false;
+                        break;
+                    }
+                    if (!ptx::mbar_wait_bounded(full(s), phase, abort_word)) {
+                        ok = false;
+                        break;
+                    }
+                    ptx::tc_fence_after_sync();
+                    const uint64_t a_desc = a_desc0 + static_cast<uint64_t>((s * stage_bytes) >> 4);
+                    const uint64_t b_desc = a_desc + (kLinearBoxBytes >> 4);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        if (EIGHT)
+                            ptx::umma_f8_ss(d_tmem, a_desc + j * 2, b_desc + j * 2, idesc, j > 0);
+                        else
+                            ptx::umma_f16_ss(d_tmem, a_desc + j * 2, b_desc + j * 2, idesc, !fresh || j > 0);
+                    }
+                    ptx::umma_commit(empty(s));
+                    if (EIGHT || k == seg.kb1 - 1) {
+                        ptx::umma_commit(acc_full(use % NBUF));
+                        use++;
+                    }
+                    if (++s == p.stages) {
+                        s = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+        }
+    }
+    else if (warp == 2) {
+        // ------------------------------------------------------------ scales
+        if (EIGHT) {
+            constexpr int PER = NMAX / 32, BATCH = 4;
+            const int     blocks_m = tiles_m;
+            int           use      = 0;
+            bool          ok       = true;
+            for (int i = 0; ok; i++) {
+                const LinearSegment seg = linear_segment(part, worker, i);
+                if (seg.tile < 0)
+                    break;
+                const LinearTile t  = locate(seg.tile);
+                const float*     sa = p.a_scales + (static_cast<size_t>(t.group) * blocks_m + t.m0 / kLinearRows) * p.kb;
+                const float*     sb = p.b_scales + t.row0;
+                float            a[BATCH], b[BATCH][PER];
+                auto fetch = [&](int k0) {
+#pragma unroll
+                    for (int u = 0; u < BATCH; u++) {
+                        const int k = min(k0 + u, seg.kb1 - 1);
+                        a[u]        = __ldg(sa + k);
+#pragma unroll
+                        for (int j = 0; j < PER; j++)
+                            b[u][j] = lane + 32 * j < t.rows ? __ldg(sb + static_cast<size_t>(k) * p.n + lane + 32 * j) : 0.0f;
+                    }
+                };
+                fetch(seg.kb0);
+#pragma unroll 1
+                for (int k0 = seg.kb0; k0 < seg.kb1 && ok; k0 += BATCH) {
+                    float v[BATCH][PER];
+#pragma unroll
+                    for (int u = 0; u < BATCH; u++)
+#pragma unroll
+                        for (int j = 0; j < PER; j++)
+                            v[u][j] = a[u] * b[u][j];
+                    if (k0 + BATCH < seg.kb1)
+                        fetch(k0 + BATCH);
+#pragma unroll
+                    for (int u = 0; u < BATCH; u++) {
+                        if (k0 + u < seg.kb1 && ok) {
+                            const int slot = use % kScaleSlots;
+                            if (use >= kScaleSlots)
+                                ok = linear_warp_wait(scale_free(slot), (use / kScaleSlots - 1) & 1, abort_word, lane);
+                            if (ok) {
+#pragma unroll
+                                for (int j = 0; j < PER; j++)
+                                    scale_ring[slot * NMAX + lane + 32 * j] = v[u][j];
+                                __syncwarp();
+                                if (lane == 0)
+                                    ptx::mbar_arrive(scale_full(slot));
+                                use++;
+                            }
+                        }
+                    }
+                }
+            }
+        }
+    }
+    else if (warp >= 4) {
+        // ------------------------------------------------------------ epilogue
+        const int      team    = (warp - 4) >> 2;
+        const int      row     = (warp & 3) * 32 + lane;  // lane of the accumulator
+        const uint32_t tmem_at = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        auto           col_of  = [&](int i) { return (2 * i + team) * CH; };
+        int            use     = 0;
+        bool           ok      = true;
+        for (int i = 0; ok; i++) {
+            const LinearSegment seg = linear_segment(part, worker, i);
+            if (seg.tile < 0)
+                break;
+            const LinearTile t = locate(seg.tile);
+            const int        n = columns(t);
+            float            acc[EIGHT ? NCH * CH : 1];
+            uint32_t         chunk[CH];
+            if (EIGHT) {
+#pragma unroll
+                for (int c = 0; c < NCH * CH; c++)
+                    acc[c] = 0.0f;
+#pragma unroll 1
+                for (int k = seg.kb0; k < seg.kb1; k++, use++) {
+                    const int slot = use % kScaleSlots, buf = use % NBUF;
+                    ok = linear_warp_wait(scale_full(slot), (use / kScaleSlots) & 1, abort_word, lane)
+                         && linear_warp_wait(acc_full(buf), (use / NBUF) & 1, abort_word, lane);
+                    if (!ok)
+                        break;
+                    ptx::tc_fence_after_sync();
+#pragma unroll
+                    for (int c = 0; c < NCH; c++) {
+                        if (col_of(c) < n) {
+                            ptx::tmem_ld_x16(tmem_at + buf * NMAX + col_of(c), chunk);
+                            ptx::tmem_ld_wait();
+                            const float4* sc = reinterpret_cast<const float4*>(scale_ring + slot * NMAX + col_of(c));
+#pragma unroll
+                            for (int j = 0; j < CH / 4; j++) {
+                                const float4 f = sc[j];
+                                acc[c * CH + 4 * j] += __uint_as_float(chunk[4 * j]) * f.x;
+                                acc[c * CH + 4 * j + 1] += __uint_as_float(chunk[4 * j + 1]) * f.y;
+                                acc[c * CH + 4 * j + 2] += __uint_as_float(chunk[4 * j + 2]) * f.z;
+                                acc[c * CH + 4 * j + 3] += __uint_as_float(chunk[4 * j + 3]) * f.w;
+                            }
+                        }
+                    }
+                    ptx::tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) {
+                        ptx::mbar_arrive(acc_free(buf));
+                        ptx::mbar_arrive(scale_free(slot));
+                    }
+                }
+            }
+            else {
+                ok = linear_warp_wait(acc_full(use % NBUF), (use / NBUF) & 1, abort_word, lane);
+                ptx::tc_fence_after_sync();
+            }
+            if (!ok)
+                break;
+            // chunk c of this warp as fp32: out of the registers, or out of TMEM
+            auto values = [&](int c, float* v) {
+                if (EIGHT) {
+#pragma unroll
+                    for (int j = 0; j < CH; j++)
+                        v[j] = acc[c * CH + j];
+                }
+                else {
+                    ptx::tmem_ld_x16(tmem_at + (use % NBUF) * NMAX + col_of(c), chunk);
+                    ptx::tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < CH; j++)
+                        v[j] = __uint_as_float(chunk[j]);
+                }
+            };
+            auto store = [&](int c, const float* v) {
+                const int m = t.m0 + row;
+                if (m >= p.m)
+                    return;
+#pragma unroll
+                for (int j = 0; j < CH; j++) {
+                    const int token = col_of(c) + j;
+                    if (token < t.rows) {
+                        const size_t at = static_cast<size_t>(t.row0 + token) * p.m + m;
+                        if (p.bf16)
+                            static_cast<__nv_bfloat16*>(p.C)[at] = __float2bfloat16_rn(v[j]);
+                        else
+                            static_cast<half*>(p.C)[at] = __float2half_rn(v[j]);
+                    }
+                }
+            };
+            if (seg.slot < 0) {
+#pragma unroll
+                for (int c = 0; c < NCH; c++)
+                    if (col_of(c) < n) {
+                        float v[CH];
+                        values(c, v);
+                        store(c, v);
+                    }
+            }
+            else {
+                // slots: [columns / 4][128 lanes] float4, so that a warp's accesses are contiguous
+                const size_t  slot4 = static_cast<size_t>(kLinearRows) * p.nt / 4;
+                float4* const slots = reinterpret_cast<float4*>(p.slots) + row;
+                float4* const mine  = slots + seg.slot * slot4;
+#pragma unroll
+                for (int c = 0; c < NCH; c++)
+                    if (col_of(c) < n) {
+                        float v[CH];
+                        values(c, v);
+#pragma unroll
+                        for (int j = 0; j < CH / 4; j++)
+                            __stcg(mine + (col_of(c) / 4 + j) * kLinearRows, make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+                    }
+                __threadfence();
+                __syncwarp();
+                unsigned  arrived = 0;
+                unsigned* counter = p.counters + seg.first * kEpilogueTeams + (warp - 4);
+                if (lane == 0)
+                    arrived = atomicAdd(counter, 1u);
+                arrived = __shfl_sync(0xffffffffu, arrived, 0);
+                if (arrived == static_cast<unsigned>(seg.last - seg.first)) {
+                    if (lane == 0)
+                        *counter = 0;  // as the next launch expects it
+                    __threadfence();
+#pragma unroll 1
+                    for (int c = 0; c < NCH; c++)
+                        if (col_of(c) < n) {
+                            float v[CH];
+#pragma unroll
+                            for (int j = 0; j < CH; j++)
+                                v[j] = 0.0f;
+#pragma unroll 1
+                            for (int w = seg.first; w <= seg.last; w++) {
+                                const float4* from = slots + linear_slot_of(part, seg, w) * slot4 + (col_of(c) / 4) * kLinearRows;
+#pragma unroll
+                                for (int j = 0; j < CH / 4; j++) {
+                                    const float4 f = __ldcg(from + j * kLinearRows);
+                                    v[4 * j] += f.x;
+                                    v[4 * j + 1] += f.y;
+                                    v[4 * j + 2] += f.z;
+                                    v[4 * j + 3] += f.w;
+                                }
+                            }
+                            store(c, v);
+                        }
+                }
+            }
+            if (!EIGHT) {
+                ptx::tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0)
+                    ptx::mbar_arrive(acc_free(use % NBUF));
+                use++;
+            }
+        }
+    }
+
+    // ---------------------------------------------------------------- exit
+    __syncwarp();
+    if (warp == 0 && lane == 0 && *abort_word != 0)  // copies still under way land before the block's memory goes
+        for (int i = max(0, issued - p.stages); i < issued; i++)
+            ptx::mbar_wait_quiet(full(i % p.stages), (i / p.stages) & 1, 10000000ull);
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    if (threadIdx.x == 0 && *abort_word != 0)
+        atomicExch(&g_linear_status, 1);
+    if (warp == 1) {
+        ptx::tc_fence_after_sync();
+        ptx::tmem_dealloc(tmem_base, 512);
+    }
+}
+
+}  // namespace spmm_b200

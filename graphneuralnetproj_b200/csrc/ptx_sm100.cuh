@@ -179,6 +179,19 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst_smem, const void* tenso
                  : "memory");
 }
 
+// The same for a 3-D tensor.
+__device__ __forceinline__ void tma_load_3d(uint32_t dst_smem, const void* tensor_map, int x, int y, int z, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                     dst_smem),
+                 "l"(tensor_map),
+                 "r"(x),
+                 "r"(y),
+                 "r"(z),
+                 "r"(bar)
+                 : "memory");
+}
+
 // The same load issued by either block of a pair (a cluster of two): the box lands in the issuing block's
 // shared memory, the bytes are counted on an mbarrier of either block (`bar_cluster`: address in the
 // cluster's shared window, see map_to_cta), which is how the partner's half of an operand is reported to
@@ -255,6 +268,21 @@ umma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, u
     asm volatile("{\n\t.reg .pred p;\n\t"
                  "setp.ne.b32 p, %4, 0;\n\t"
                  "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d_tmem),
+                 "l"(a_desc),
+                 "l"(b_desc),
+                 "r"(idesc),
+                 "r"(accumulate),
+                 "r"(0u)
+                 : "memory");
+}
+
+// The same for 8-bit floating-point inputs (K = 32 per instruction).
+__device__ __forceinline__ void
+umma_f8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d_tmem),
                  "l"(a_desc),
                  "l"(b_desc),
                  "r"(idesc),
@@ -459,6 +487,9 @@ __host__ __device__ constexpr uint32_t make_idesc_f16_f32(int m, int n, bool a_m
            | (static_cast<uint32_t>(a_mn_major) << 15) | (static_cast<uint32_t>(b_mn_major) << 16)
            | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
+
+// The operand formats of an instruction descriptor (both operands alike): 0 is f16 in kind::f16 and e4m3 in kind::f8f6f4.
+constexpr uint32_t kIdescBf16 = (1u << 7) | (1u << 10);
 
 constexpr uint32_t kIdescSparse = 1u << 2;  // A is 2:4-compressed, metadata in TMEM
 

@@ -11,6 +11,7 @@
 #include "../../include/SpMM_API.cuh"
 #include "../../include/spmm_b200.h"
 #include "host_threads.h"
+#include "linear_api.h"
 #include "spmm_decode_kernel.cuh"
 #include "spmm_pair_kernel.cuh"
 #include "spmm_structured_kernel.cuh"
@@ -981,7 +982,8 @@ int spmm_b200_device_status(int reset)
             cudaMemset(counters, 0, sizeof(spmm_b200::g_row_arrivals));
         cudaDeviceSynchronize();
     }
-    return status;
+    const int linear = spmm_b200::linear_status(reset);
+    return status != 0 ? status : linear;
 }
 
 namespace spmm_b200 {

@@ -114,6 +114,19 @@ def _load():
     lib.spmm_b200_suggest_split_k.restype = ctypes.c_int
     lib.spmm_b200_write_rank_lists.argtypes = [ctypes.c_char_p, ctypes.c_int, ctypes.c_int, _i32p, _i32p]
     lib.spmm_b200_write_rank_lists.restype = ctypes.c_int
+    vp, ci, sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
+    lib.spmm_b200_quantize_fp8.argtypes = [vp, vp] + [ci] * 5 + [vp, vp]
+    lib.spmm_b200_quantize_fp8.restype = ci
+    lib.spmm_b200_linear_workspace_bytes.argtypes = [ci] * 5
+    lib.spmm_b200_linear_workspace_bytes.restype = sz
+    lib.spmm_b200_fp8_linear.argtypes = [vp] * 6 + [ci] * 4 + [vp, sz]
+    lib.spmm_b200_fp8_linear.restype = ci
+    lib.spmm_b200_grouped_linear.argtypes = [vp] * 4 + [ci, vp] + [ci] * 4 + [vp, sz]
+    lib.spmm_b200_grouped_linear.restype = ci
+    lib.spmm_b200_grouped_fp8_linear.argtypes = [vp] * 6 + [ci, vp] + [ci] * 4 + [vp, sz]
+    lib.spmm_b200_grouped_fp8_linear.restype = ci
+    lib.spmm_b200_linear_plan.argtypes = [ci] * 6 + [_i32p]
+    lib.spmm_b200_linear_plan.restype = ci
     lib.spmm_b200_plan.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_long, _i32p, _i32p, _i32p]
     lib.spmm_b200_plan.restype = ctypes.c_int
     lib.GenSparseMatrixBinFile.argtypes = [ctypes.c_char_p, ctypes.c_int, ctypes.c_int, ctypes.c_char_p, ctypes.c_char_p,
@@ -257,6 +270,125 @@ def spmm_own_scratch(stream, Compressed_A, TileOffsets, B, C, M_Global, N_Global
     handle = stream if isinstance(stream, int) else stream.cuda_stream
     return LIB.spmm_b200_spmm_own_scratch(ctypes.c_void_p(handle), _dev_ptr(Compressed_A), _dev_ptr(TileOffsets),
                                           _dev_ptr(B), _dev_ptr(C), M_Global, N_Global, K_Global)
+
+
+def _operands(stream, *operands):
+    """(stream handle, [device pointers]) after checking each (name, tensor, dtypes, elements): a contiguous CUDA tensor
+    of the stream's device, which is the current one, of one of the types and with exactly that many elements."""
+    import torch
+    device = torch.cuda.current_device()
+    if stream is None:
+        stream = torch.cuda.current_stream()
+    if not isinstance(stream, int):
+        if stream.device.index != device:
+            raise ValueError("the stream belongs to device %s, the current device is %d" % (stream.device, device))
+        stream = stream.cuda_stream
+    pointers = []
+    for name, t, dtypes, elements in operands:
+        if not t.is_cuda or t.get_device() != device:
+            raise ValueError("%s must be a CUDA tensor on the current device" % name)
+        if t.dtype not in dtypes:
+            raise ValueError("%s has type %s, expected one of %s" % (name, t.dtype, ", ".join(map(str, dtypes))))
+        if t.numel() != elements:
+            raise ValueError("%s has %d elements, expected %d" % (name, t.numel(), elements))
+        if not t.is_contiguous():
+            raise ValueError("%s must be contiguous" % name)
+        pointers.append(t.data_ptr())
+    return stream, pointers
+
+
+def _types():
+    import torch
+    return (torch.float16, torch.bfloat16), (torch.float8_e4m3fn, torch.uint8), (torch.float32,), (torch.int32,)
+
+
+def _workspace(workspace):
+    """(pointer, bytes) of a workspace tensor, or of none."""
+    if workspace is None:
+        return None, 0
+    import torch
+    if not workspace.is_contiguous() or not workspace.is_cuda or workspace.get_device() != torch.cuda.current_device():
+        raise ValueError("the workspace must be a contiguous CUDA tensor on the current device")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def _blocks(n):
+    return -(-n // 128)
+
+
+def quantize_fp8(stream, X, codes, scales, block_rows):
+    """e4m3 codes and fp32 scales of X ([rows][cols], or [groups][rows][cols] for block_rows = 128), fp16 or bf16.
+
+    block_rows = 1: one scale per 1 x 128 block, scales[ceil(cols / 128)][rows] (activations); block_rows = 128: one per
+    128 x 128 block, scales[(groups)][ceil(rows / 128)][ceil(cols / 128)] (weights).  codes: float8_e4m3fn or uint8, the
+    shape of X.  See spmm_b200_quantize_fp8 in include/spmm_b200.h for the rounding.  Returns a cudaError_t as an int."""
+    wide, eight, single, _ = _types()
+    if X.dim() not in (2, 3) or block_rows not in (1, 128) or (block_rows == 1 and X.dim() != 2):
+        raise ValueError("X must be [rows][cols], or [groups][rows][cols] with block_rows = 128; block_rows 1 or 128")
+    groups = X.shape[0] if X.dim() == 3 else 1
+    rows, cols = X.shape[-2:]
+    blocks = _blocks(cols) * (rows if block_rows == 1 else groups * _blocks(rows))
+    handle, (x, c, s) = _operands(stream, ("X", X, wide, X.numel()), ("codes", codes, eight, X.numel()), ("scales", scales, single, blocks))
+    return LIB.spmm_b200_quantize_fp8(handle, x, int(X.dtype is wide[1]), groups, rows, cols, block_rows, c, s)
+
+
+def linear_workspace_bytes(groups, M_Global, N_Global, K_Global, eight_bit):
+    """Bytes of (once zero-filled) workspace for fp8_linear (groups = 1), grouped_linear and grouped_fp8_linear."""
+    return int(LIB.spmm_b200_linear_workspace_bytes(groups, M_Global, N_Global, K_Global, int(eight_bit)))
+
+
+def fp8_linear(stream, A, A_scales, B, B_scales, C, M_Global, N_Global, K_Global, workspace):
+    """C[N][M] = B[N][K] * A[M][K]^T from e4m3 codes and the scales quantize_fp8 gives (weights: block_rows = 128,
+    activations: block_rows = 1); C fp16 or bf16.  workspace: a CUDA tensor, zero-filled once, of
+    linear_workspace_bytes(1, M, N, K, True) bytes, or None.  Returns a cudaError_t as an int; asynchronous."""
+    wide, eight, single, _ = _types()
+    M, N, K = M_Global, N_Global, K_Global
+    handle, (a, sa, b, sb, c) = _operands(stream, ("A", A, eight, M * K), ("A_scales", A_scales, single, _blocks(M) * _blocks(K)),
+                                          ("B", B, eight, N * K), ("B_scales", B_scales, single, _blocks(K) * N), ("C", C, wide, N * M))
+    ws, ws_bytes = _workspace(workspace)
+    return LIB.spmm_b200_fp8_linear(handle, a, sa, b, sb, c, int(C.dtype is wide[1]), M, N, K, ws, ws_bytes)
+
+
+def grouped_linear(stream, A, B, C, group_offsets, groups, M_Global, N_Global, K_Global, workspace):
+    """C[t] = B[t] * A[g]^T for the tokens t of group g, group_offsets[g] <= t < group_offsets[g + 1] (int32, on the
+    device); A[groups][M][K], B[N][K], C[N][M], all fp16 or all bf16.  Rows of C outside all groups stay as they were.
+    workspace: linear_workspace_bytes(groups, M, N, K, False) bytes, zero-filled once, or None."""
+    wide, _, _, index = _types()
+    M, N, K = M_Global, N_Global, K_Global
+    if B.dtype is not A.dtype or C.dtype is not A.dtype:
+        raise ValueError("A, B and C must have the same type")
+    handle, (a, b, c, o) = _operands(stream, ("A", A, wide, groups * M * K), ("B", B, wide, N * K), ("C", C, wide, N * M),
+                                     ("group_offsets", group_offsets, index, groups + 1))
+    ws, ws_bytes = _workspace(workspace)
+    return LIB.spmm_b200_grouped_linear(handle, a, b, c, int(C.dtype is wide[1]), o, groups, M, N, K, ws, ws_bytes)
+
+
+def grouped_fp8_linear(stream, A, A_scales, B, B_scales, C, group_offsets, groups, M_Global, N_Global, K_Global, workspace):
+    """grouped_linear from e4m3 codes and scales: A[groups][M][K] with A_scales[groups][ceil(M / 128)][ceil(K / 128)],
+    B[N][K] with B_scales[ceil(K / 128)][N]; C fp16 or bf16."""
+    wide, eight, single, index = _types()
+    M, N, K = M_Global, N_Global, K_Global
+    handle, (a, sa, b, sb, c, o) = _operands(
+        stream, ("A", A, eight, groups * M * K), ("A_scales", A_scales, single, groups * _blocks(M) * _blocks(K)),
+        ("B", B, eight, N * K), ("B_scales", B_scales, single, _blocks(K) * N), ("C", C, wide, N * M),
+        ("group_offsets", group_offsets, index, groups + 1))
+    ws, ws_bytes = _workspace(workspace)
+    return LIB.spmm_b200_grouped_fp8_linear(handle, a, sa, b, sb, c, int(C.dtype is wide[1]), o, groups, M, N, K, ws, ws_bytes)
+
+
+def linear_plan(tiles, kb, workers, overhead):
+    """How the linear layers share out `tiles` tiles of `kb` k-blocks: per worker a list of (tile, first k-block, past the
+    last, workspace slot or -1, first and last worker of the tile, slot the piece is read from)."""
+    plan, segment = [], (ctypes.c_int * 7)()
+    for worker in range(workers):
+        plan.append([])
+        while True:
+            if LIB.spmm_b200_linear_plan(tiles, kb, workers, overhead, worker, len(plan[-1]), segment) != 0:
+                raise ValueError("no such plan")
+            if segment[0] < 0:
+                break
+            plan[-1].append(tuple(segment))
+    return plan
 
 
 def set_weights_constant(constant=True):

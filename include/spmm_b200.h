@@ -318,6 +318,94 @@ void spmm_b200_decompose(const uint16_t* A, uint16_t* A1, uint16_t* A2, int leng
 int spmm_b200_pack_a1(const uint16_t* A1, int M, int K, void** values, void** metadata);
 void spmm_b200_decompose_v1(const uint16_t* A, uint16_t* A1, uint16_t* A2, int length);
 
+/* ------------------------------------------------------------------------------------------------
+ * Linear layers on dense weights: 8 bits per weight, and one matrix per group of tokens (experts).
+ * No counterpart in the reference.  Layouts are those of the token-major SpMM: A[M][K] weights (M output
+ * features), B[N][K] activations (one token per row), C[N][M] results; all row-major and contiguous.
+ *
+ * 16-bit values are fp16 or bf16 (SPMM_B200_FP16 / SPMM_B200_BF16).  8-bit values are e4m3 codes with fp32
+ * scales, KB = ceil(K / 128) of them along K:
+ *   weights      one scale per 128 x 128 block:            A_scales[groups][ceil(M / 128)][KB]
+ *   activations  one per token and 128 features of it:     B_scales[KB][N]  (tokens contiguous)
+ * A value is code * scale.  Products of codes are summed in fp32 by the tensor core over 128 features, times
+ * the two scales, and summed in fp32 over the KB blocks; C is rounded once.
+ *
+ * All calls are asynchronous on `stream`, allocate nothing and may be captured in a CUDA graph (make the first
+ * call on a device outside a capture, as for the SpMM).  A, B, codes and workspaces start on 16-byte boundaries.
+ * N = 0 returns at once.  They return a cudaError_t as an int; cudaErrorInvalidValue for sizes, types or
+ * pointers that are not as described here, before anything is launched. */
+#define SPMM_B200_FP16 0
+#define SPMM_B200_BF16 1
+
+/* Codes and scales of X[groups][rows][cols] (cols a multiple of 16).  block_rows = 128: blocks of 128 x 128
+ * (weights; scales[groups][ceil(rows / 128)][ceil(cols / 128)]).  block_rows = 1, groups = 1: blocks of 1 x 128
+ * (activations; scales[ceil(cols / 128)][rows]).  The scale is max(amax / 448, 2^-64), amax over the block's
+ * finite elements; the code is the e4m3 value nearest to x / scale (the exact quotient; ties to even).  Infinite
+ * and NaN elements become NaN. */
+int spmm_b200_quantize_fp8(
+    void* stream, const void* X, int X_type, int groups, int rows, int cols, int block_rows, void* codes, float* scales);
+
+/* Bytes of workspace with which the three products below cut the K range of tiles between SMs where that helps
+ * (few tokens, or a last round of tiles that does not fill the GPU); 0 for sizes they refuse.  With less, or
+ * none, they run without cutting, at the same results within the rounding of the sums.  A workspace is filled
+ * with zeros once, before its first use; every call leaves it ready for the next, of any size it is large enough
+ * for.  Calls that may run at the same time need different workspaces (also calls captured in graphs that may). */
+size_t spmm_b200_linear_workspace_bytes(int groups, int M_Global, int N_Global, int K_Global, int eight_bit);
+
+/* C = B * A^T from codes and scales.  K a multiple of 16; any M and N.  C_type: type of C. */
+int spmm_b200_fp8_linear(void*        stream,
+                         const void*  A,
+                         const float* A_scales,
+                         const void*  B,
+                         const float* B_scales,
+                         void*        C,
+                         int          C_type,
+                         int          M_Global,
+                         int          N_Global,
+                         int          K_Global,
+                         void*        workspace,
+                         size_t       workspace_bytes);
+
+/* One matrix per group of consecutive tokens: C[t] = B[t] * A[g]^T for group_offsets[g] <= t < group_offsets[g + 1],
+ * g = 0 .. groups - 1 (1 .. 1024), A[groups][M][K].  group_offsets: groups + 1 ints in device memory, not
+ * decreasing, within 0 .. N_Global, read when the kernel runs (so an earlier kernel in the stream may write them);
+ * groups may be empty.  Rows of C before the first group and behind the last are left as they were.  Borders
+ * outside 0 .. N_Global are taken as the nearest one inside, so that a corrupt table gives wrong rows but touches
+ * nothing outside B and C.  A, B and C of the same type; K a multiple of 8. */
+int spmm_b200_grouped_linear(void*       stream,
+                             const void* A,
+                             const void* B,
+                             void*       C,
+                             int         type,
+                             const int*  group_offsets,
+                             int         groups,
+                             int         M_Global,
+                             int         N_Global,
+                             int         K_Global,
+                             void*       workspace,
+                             size_t      workspace_bytes);
+
+/* The same from codes and scales: A_scales[groups][ceil(M / 128)][KB], B_scales[KB][N]; K a multiple of 16. */
+int spmm_b200_grouped_fp8_linear(void*        stream,
+                                 const void*  A,
+                                 const float* A_scales,
+                                 const void*  B,
+                                 const float* B_scales,
+                                 void*        C,
+                                 int          C_type,
+                                 const int*   group_offsets,
+                                 int          groups,
+                                 int          M_Global,
+                                 int          N_Global,
+                                 int          K_Global,
+                                 void*        workspace,
+                                 size_t       workspace_bytes);
+
+/* Segment `index` of the share of tiles that block `worker` of a linear layer gets (for tests of the host logic):
+ * segment[7] = tile (-1: no such segment), first and past-the-last k-block, workspace slot or -1, first and last
+ * worker with a piece of the tile, and the slot the adding worker reads this piece from. */
+int spmm_b200_linear_plan(int tiles, int kb, int workers, int overhead, int worker, int index, int* segment);
+
 /* Device-side status of the current device: 0 = ok, 1 = a bounded wait inside a
  * kernel gave up.  Synchronises the device.  With reset != 0 the status and the
  * arrival counters are cleared afterwards.  No counterpart in the reference,

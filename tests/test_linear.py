@@ -1,0 +1,80 @@
+"""Host side of the linear layers on dense weights: how tiles are shared out, workspace sizes, refusals without a GPU."""
+import ctypes
+import random
+
+import pytest
+
+
+@pytest.mark.parametrize("workers", [148, 74, 1, 13])
+@pytest.mark.parametrize("overhead", [-1, 0, 4, 20])
+def test_plan_covers_every_k_block_once(sp, workers, overhead):
+    rng = random.Random(workers * 100 + overhead)
+    for tiles, kb in [(0, 5), (1, 1), (1, 300), (workers, 7), (workers + 1, 64), (2 * workers - 1, 3)] + \
+            [(rng.randint(1, 500), rng.randint(1, 300)) for _ in range(30)]:
+        pieces, slots = {}, set()
+        for worker, segments in enumerate(sp.linear_plan(tiles, kb, workers, overhead)):
+            for tile, k0, k1, slot, first, last, read_from in segments:
+                assert 0 <= tile < tiles and 0 <= k0 < k1 <= kb
+                pieces.setdefault(tile, []).append((k0, k1, worker, slot, first, last))
+                if slot >= 0:  # parked where the adding worker looks for it, and nobody else parks there
+                    assert slot == read_from and slot < 2 * workers and slot not in slots
+                    slots.add(slot)
+        assert sorted(pieces) == list(range(tiles))
+        counters = set()
+        for parts in pieces.values():
+            parts.sort()
+            assert parts[0][0] == 0 and parts[-1][1] == kb and all(a[1] == b[0] for a, b in zip(parts, parts[1:]))
+            assert (len(parts) == 1) == (parts[0][3] < 0)
+            owners = [p[2] for p in parts]
+            assert owners == list(range(owners[0], owners[-1] + 1)) and len(owners) <= 17
+            assert all(p[4] == owners[0] and p[5] == owners[-1] for p in parts)
+            if len(parts) > 1:  # arrivals are counted under the first owner
+                assert owners[0] not in counters
+                counters.add(owners[0])
+        if overhead < 0:
+            assert not slots
+
+
+def test_plan_evens_out_few_tiles(sp):
+    """72 tiles of 72 k-blocks on 148 workers: nobody has more than its share, rounded up."""
+    plan = sp.linear_plan(72, 72, 148, 4)
+    assert max(sum(s[2] - s[1] for s in segments) for segments in plan) == -(-72 * 72 // 148)
+
+
+def test_workspace_bytes(sp):
+    assert sp.linear_workspace_bytes(1, 9216, 16, 9216, True) > 0
+    assert sp.linear_workspace_bytes(64, 2048, 96, 4096, False) > 0
+    for bad in [(0, 128, 16, 128, True), (1025, 128, 16, 128, True), (1, 0, 16, 128, True), (1, 128, -1, 128, True), (1, 128, 16, 0, True),
+                (1, 128, 16, 24, True), (1, 128, 16, 12, False)]:
+        assert sp.linear_workspace_bytes(*bad) == 0, bad
+
+
+def test_c_boundary_refuses_before_any_cuda_call(sp):
+    lib, p, odd = sp.spmm_api.LIB, ctypes.c_void_p(4096), ctypes.c_void_p(4100)
+    quant = lib.spmm_b200_quantize_fp8
+    assert quant(None, p, 0, 1, 0, 128, 1, p, p) == 0  # nothing to do
+    for args in [(p, 2, 1, 4, 128, 1, p, p), (p, 0, 0, 4, 128, 1, p, p), (p, 0, 2, 4, 128, 1, p, p), (p, 0, 1, -1, 128, 1, p, p),
+                 (p, 0, 1, 4, 120, 1, p, p), (p, 0, 1, 4, 0, 1, p, p), (p, 0, 1, 4, 128, 64, p, p), (None, 0, 1, 4, 128, 1, p, p),
+                 (p, 0, 1, 4, 128, 1, None, p), (p, 0, 1, 4, 128, 1, p, None), (odd, 0, 1, 4, 128, 1, p, p), (p, 0, 1, 4, 128, 1, odd, p)]:
+        assert quant(None, *args) == 1, args
+    fp8 = lib.spmm_b200_fp8_linear
+    assert fp8(None, None, None, None, None, None, 0, 128, 0, 128, None, 0) == 0
+    good = [p, p, p, p, p, 0, 128, 16, 128, None, 0]
+    for at, value in [(0, None), (1, None), (2, None), (3, None), (4, None), (0, odd), (2, odd), (5, 2), (5, -1), (6, 0), (7, -1), (8, 0),
+                      (8, 120), (9, odd), (4, ctypes.c_void_p(4097))]:
+        args = list(good)
+        args[at] = value
+        assert fp8(None, *args) == 1, (at, value)
+    grouped = lib.spmm_b200_grouped_linear
+    good = [p, p, p, 1, p, 4, 128, 16, 128, None, 0]
+    for at, value in [(0, None), (1, None), (2, None), (3, 2), (4, None), (4, ctypes.c_void_p(4098)), (5, 0), (5, 1025), (6, 0), (7, -1),
+                      (8, 0), (8, 12), (0, odd), (1, odd)]:
+        args = list(good)
+        args[at] = value
+        assert grouped(None, *args) == 1, (at, value)
+    grouped8 = lib.spmm_b200_grouped_fp8_linear
+    good = [p, p, p, p, p, 0, p, 4, 128, 16, 128, None, 0]
+    for at, value in [(0, None), (1, None), (3, None), (4, None), (6, None), (5, 3), (7, 0), (8, -128), (10, 24)]:
+        args = list(good)
+        args[at] = value
+        assert grouped8(None, *args) == 1, (at, value)

@@ -1,0 +1,400 @@
+"""The 8-bit block-scaled and grouped linear layers against their definitions in 64 bits.
+
+Tolerance of a product, from the arithmetic alone: the values that codes and scales stand for are exact in 64 bits; the
+kernel's sums are fp32.  A sum of K products in fp32, in whatever order and with each addition cut off rather than rounded
+(what a tensor core may do), is off by at most K * 2^-23 * sum |a b|; the scales multiply in with three more roundings
+(their product, the product with the block's sum, the addition), which the same bound with K + 4 covers; C is rounded
+once, by half a step of its type (2^-11 or 2^-8 of the value, 2^-25 where fp16 is subnormal)."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+HALF_STEP = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+E4M3 = np.array([i * 2.0 ** -9 for i in range(8)] + [(8 + f) * 2.0 ** (e - 3) for e in range(-6, 9) for f in range(8)][:119])
+
+
+@pytest.fixture(scope="module", autouse=True)
+def cuda():
+    assert torch.cuda.is_available(), "these tests need a CUDA device"
+
+
+def rng(*seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(hash(seed) % (1 << 31))
+    return g
+
+
+def kb_of(k):
+    return -(-k // 128)
+
+
+def random_operands(groups, m, n, k, dtype, seed):
+    """Random codes with random scales (8 bits) or random values: tensors for the call and their fp64 values."""
+    g = rng(groups, m, n, k, seed)
+    a = torch.randn((groups, m, k), device="cuda", generator=g)
+    b = torch.randn((n, k), device="cuda", generator=g)
+    if dtype is not None:
+        a, b = a.to(dtype), b.to(dtype)
+        return a, None, b, None, a.double(), b.double()
+    a8, b8 = (a * 30).to(torch.float8_e4m3fn), (b * 30).to(torch.float8_e4m3fn)
+    sa = torch.rand((groups, kb_of(m), kb_of(k)), device="cuda", generator=g) + 0.5
+    sb = torch.rand((kb_of(k), n), device="cuda", generator=g) * 0.01 + 1e-3
+    av = a8.double() * sa.double().repeat_interleave(128, 1)[:, :m].repeat_interleave(128, 2)[:, :, :k]
+    bv = b8.double() * sb.double().t().repeat_interleave(128, 1)[:, :k]
+    return a8, sa, b8, sb, av, bv
+
+
+def integer_operands(groups, m, n, k, dtype, seed):
+    """Small whole numbers and powers of two as scales: every partial sum is exact, so C must be too.  Values -1, 0, 1 on
+    a tenth of the places of A: sums stay below 2^8 with room, exact in bf16 as well."""
+    g = rng(groups, m, n, k, seed, 1)
+    a = (torch.rand((groups, m, k), device="cuda", generator=g) < 40.0 / k).float() * torch.randint(-1, 2, (groups, m, k), device="cuda", generator=g)
+    b = torch.randint(-1, 2, (n, k), device="cuda", generator=g).float()
+    if dtype is not None:
+        return a.to(dtype), None, b.to(dtype), None, a.double(), b.double()
+    sa = torch.full((groups, kb_of(m), kb_of(k)), 0.5, device="cuda")
+    sb = torch.full((kb_of(k), n), 2.0, device="cuda")
+    return a.to(torch.float8_e4m3fn), sa, b.to(torch.float8_e4m3fn), sb, a.double(), b.double()
+
+
+def workspace_for(sp, groups, m, n, k, eight):
+    return torch.zeros(sp.linear_workspace_bytes(groups, m, n, k, eight), dtype=torch.uint8, device="cuda")
+
+
+def call(sp, a, sa, b, sb, c, offsets, groups, m, n, k, ws, stream=None):
+    if offsets is None:
+        return sp.fp8_linear(stream, a, sa, b, sb, c, m, n, k, ws)
+    if sa is None:
+        return sp.grouped_linear(stream, a, b, c, offsets, groups, m, n, k, ws)
+    return sp.grouped_fp8_linear(stream, a, sa, b, sb, c, offsets, groups, m, n, k, ws)
+
+
+def check(c, av, bv, offsets, k, out, exact=False):
+    """c against the definition; rows outside all groups still hold 7."""
+    n, m = c.shape
+    borders = [0, n] if offsets is None else offsets
+    covered = torch.zeros(n, dtype=torch.bool, device="cuda")
+    for e in range(len(borders) - 1):
+        rows = slice(borders[e], borders[e + 1])
+        if borders[e + 1] <= borders[e]:
+            continue
+        covered[rows] = True
+        want = bv[rows] @ av[e].t()
+        got = c[rows].double()
+        if exact:
+            assert torch.equal(got, want), "group %d" % e
+            continue
+        size = bv[rows].abs() @ av[e].abs().t()
+        bound = (k + 4) * 2.0 ** -23 * size + HALF_STEP[out] * want.abs() * 1.001 + 2.0 ** -25
+        worst = ((got - want).abs() / bound).max().item()
+        assert worst <= 1.0, "group %d: %.3f of the bound" % (e, worst)
+    assert bool((c[~covered].double() == 7).all())
+
+
+def run_case(sp, groups, m, n, k, dtype, out, offsets, with_workspace, make, exact):
+    a, sa, b, sb, av, bv = make(groups, m, n, k, dtype, 5)
+    c = torch.full((n, m), 7.0, dtype=out, device="cuda")
+    ws = workspace_for(sp, groups, m, n, k, dtype is None) if with_workspace else None
+    off = None if offsets is None else torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    assert call(sp, a, sa, b, sb, c, off, groups, m, n, k, ws) == 0
+    torch.cuda.synchronize()
+    assert sp.device_status() == 0
+    check(c, av, bv, offsets, k, out, exact)
+
+
+DENSE = [(128, 1, 128), (1, 1, 16), (130, 17, 144), (1032, 24, 1040), (257, 129, 272), (384, 300, 2048), (2304, 16, 4608), (1000, 64, 8192),
+         (128, 3, 36864), (640, 513, 640), (7168, 40, 1024), (4104, 1031, 528)]
+
+
+@pytest.mark.parametrize("make", [integer_operands, random_operands], ids=["integers", "random"])
+@pytest.mark.parametrize("with_workspace", [True, False], ids=["workspace", "alone"])
+@pytest.mark.parametrize("out", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("m,n,k", DENSE)
+def test_fp8_linear(sp, m, n, k, out, with_workspace, make):
+    run_case(sp, 1, m, n, k, None, out, None, with_workspace, make, make is integer_operands)
+
+
+def borders(sizes, start=0):
+    return [start] + [start + int(x) for x in np.cumsum(sizes)]
+
+
+GROUPED = [  # m, n, k, group sizes, first row
+    (128, 1, 128, [1], 0),
+    (128, 4, 64, [0, 0, 4, 0], 0),
+    (200, 37, 272, [5, 0, 17, 1, 14], 0),           # odd sizes
+    (136, 50, 1040, [3, 2, 40], 2),                 # rows before the first group and behind the last
+    (1032, 700, 528, [0, 300, 129, 1, 256, 0, 14], 0),
+    (256, 16, 4096, [1] * 16, 0),                   # a token each, K cut between blocks
+    (520, 2000, 144, [0] * 30 + [1990] + [0] * 33, 5),  # one group has nearly everything
+    (64, 1024, 48, [1] * 1024, 0),                  # as many groups as there may be
+    (384, 9, 2064, [0, 0, 0], 4),                   # nothing to do
+]
+
+
+@pytest.mark.parametrize("make", [integer_operands, random_operands], ids=["integers", "random"])
+@pytest.mark.parametrize("kind", ["fp16", "bf16", "e4m3-fp16", "e4m3-bf16"])
+@pytest.mark.parametrize("case", range(len(GROUPED)))
+def test_grouped(sp, case, kind, make):
+    m, n, k, sizes, start = GROUPED[case]
+    out = torch.bfloat16 if kind.endswith("bf16") else torch.float16
+    dtype = None if kind.startswith("e4m3") else out
+    for with_workspace in (True, False):
+        run_case(sp, len(sizes), m, n, k, dtype, out, borders(sizes, start), with_workspace, make, make is integer_operands)
+
+
+@pytest.mark.parametrize("eight", [True, False], ids=["e4m3", "fp16"])
+def test_repeated_calls_are_bitwise_reproducible(sp, eight):
+    """Tiles cut between blocks are added in a fixed order; the workspace is ready for the next call, of another size too."""
+    ws = workspace_for(sp, 4, 1152, 40, 9216, eight)
+    results = {}
+    for turn in range(3):
+        for n, k in ((40, 9216), (7, 4096)):
+            m, sizes = 1152, [n - 4, 0, 3, 1]
+            a, sa, b, sb, _, _ = random_operands(4, m, n, k, None if eight else torch.float16, 9)
+            c = torch.zeros((n, m), dtype=torch.float16, device="cuda")
+            off = torch.tensor(borders(sizes), dtype=torch.int32, device="cuda")
+            assert call(sp, a, sa, b, sb, c, off, 4, m, n, k, ws) == 0
+            first = results.setdefault(n, c)
+            assert torch.equal(first, c), turn
+
+
+def test_values_outside_a_group_do_not_reach_it(sp):
+    """NaN in the rows of other groups, behind the last group, and in the weights of an empty group."""
+    m, n, k, sizes = 192, 60, 256, [20, 0, 21]
+    for dtype in (None, torch.bfloat16):
+        a, sa, b, sb, av, bv = random_operands(3, m, n, k, dtype, 3)
+        a, b = a.clone(), b.clone()
+        bits = torch.uint8 if dtype is None else torch.int16
+        a[1].view(bits).fill_(0x7f if dtype is None else 0x7fff)
+        b[41:].view(bits).fill_(0x7f if dtype is None else 0x7fff)
+        b[20:41].view(bits)[3, 5] = 0x7f if dtype is None else 0x7fff
+        c = torch.full((n, m), 7.0, dtype=torch.bfloat16, device="cuda")
+        off = torch.tensor(borders(sizes), dtype=torch.int32, device="cuda")
+        assert call(sp, a, sa, b, sb, c, off, 3, m, n, k, workspace_for(sp, 3, m, n, k, dtype is None)) == 0
+        assert bool(c[23].isnan().all())
+        c[23] = (bv[23] @ av[2].t()).to(c.dtype)
+        check(c, av, bv, borders(sizes), k, torch.bfloat16)
+
+
+def test_corrupt_group_borders_touch_nothing_outside(sp):
+    m, n, k, groups = 136, 40, 128, 4
+    a, sa, b, sb, _, _ = random_operands(groups, m, n, k, None, 4)
+    for table in ([-5, 3, 2000000000, 10, 41], [40, 30, 20, 10, 0], [-1, -2, -3, -4, -5], [2147483647, -2147483648, 2147483647, 0, 100]):
+        whole = torch.full((3 * n, m), 7.0, dtype=torch.float16, device="cuda")
+        off = torch.tensor(table, dtype=torch.int32, device="cuda")
+        assert call(sp, a, sa, b, sb, whole[n:2 * n], off, groups, m, n, k, None) == 0
+        torch.cuda.synchronize()
+        assert sp.device_status() == 0
+        assert bool((whole[:n] == 7).all()) and bool((whole[2 * n:] == 7).all())
+
+
+def test_far_offsets(sp):
+    """Weights and results beyond 2^31 elements."""
+    groups, m, k, n = 9, 16384, 16384, 3
+    a = torch.zeros((groups, m, k), dtype=torch.float8_e4m3fn, device="cuda")
+    a.view(torch.uint8)[8, m - 1, k - 16:] = 0x38  # 1.0
+    sa = torch.ones((groups, m // 128, k // 128), device="cuda")
+    b, sb = torch.ones((n, k), device="cuda").to(torch.float8_e4m3fn), torch.ones((k // 128, n), device="cuda")
+    c = torch.zeros((n, m), dtype=torch.float16, device="cuda")
+    off = torch.tensor([0] * 9 + [n], dtype=torch.int32, device="cuda")
+    assert call(sp, a, sa, b, sb, c, off, groups, m, n, k, workspace_for(sp, groups, m, n, k, True)) == 0
+    assert bool((c[:, m - 1] == 16).all()) and bool((c[:, :m - 1] == 0).all())
+    del a
+    m, n, k = 65544, 32896, 16
+    a, sa, b, sb, av, bv = integer_operands(1, m, n, k, None, 6)
+    c = torch.full((n, m), 7.0, dtype=torch.float16, device="cuda")
+    assert call(sp, a, sa, b, sb, c, None, 1, m, n, k, None) == 0
+    for rows in (slice(0, 130), slice(n - 130, n)):
+        assert torch.equal(c[rows].double(), bv[rows] @ av[0].t())
+
+
+def test_two_streams_at_once_and_graph_replay(sp):
+    m, k, sizes = 1152, 4608, [9, 0, 30]
+    n = sum(sizes)
+    off = torch.tensor(borders(sizes), dtype=torch.int32, device="cuda")
+    jobs = []
+    for seed, dtype in ((1, None), (2, torch.float16)):
+        a, sa, b, sb, av, bv = random_operands(3, m, n, k, dtype, seed)
+        jobs.append((a, sa, b, sb, torch.full((n, m), 7.0, dtype=torch.float16, device="cuda"), workspace_for(sp, 3, m, n, k, dtype is None), av, bv))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):
+        for s, (a, sa, b, sb, c, ws, _, _) in zip(streams, jobs):
+            assert call(sp, a, sa, b, sb, c, off, 3, m, n, k, ws, s) == 0
+    torch.cuda.synchronize()
+    assert sp.device_status() == 0
+    for a, sa, b, sb, c, ws, av, bv in jobs:
+        check(c, av, bv, borders(sizes), k, torch.float16)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for a, sa, b, sb, c, ws, _, _ in jobs:
+            assert call(sp, a, sa, b, sb, c, off, 3, m, n, k, ws) == 0
+    other = [30, 9, 0]  # the borders are read when the graph runs
+    for table in (sizes, other, sizes):
+        off.copy_(torch.tensor(borders(table), dtype=torch.int32))
+        for job in jobs:
+            job[4].fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, sa, b, sb, c, ws, av, bv in jobs:
+            check(c, av, bv, borders(table), k, torch.float16)
+
+
+# ---------------------------------------------------------------- quantiser
+def reference_codes(x, block_rows):
+    """(values, scales) by the definition: the e4m3 value nearest to x / scale, ties to the even code."""
+    rows, cols = x.shape
+    kb, rb = kb_of(cols), -(-rows // block_rows)
+    mag = np.where(np.isfinite(x), np.abs(x), 0.0)
+    full = np.zeros((rb * block_rows, kb * 128))
+    full[:rows, :cols] = mag
+    top = full.reshape(rb, block_rows, kb, 128).max(axis=(1, 3))
+    scales = np.maximum((top / 448.0).astype(np.float32), np.float32(2.0 ** -64))
+    per = np.repeat(np.repeat(scales.astype(np.float64), block_rows, 0)[:rows], 128, 1)[:, :cols]
+    y = mag / per
+    above = np.minimum(np.searchsorted(E4M3, y), 126)
+    below = np.maximum(above - 1, 0)
+    up, down = E4M3[above] - y, y - E4M3[below]
+    value = np.where((up < down) | ((up == down) & (above % 2 == 0)), E4M3[above], E4M3[below])
+    return np.where(np.isfinite(x), np.copysign(value, x), np.nan), scales
+
+
+def quantize(sp, x, block_rows):
+    rows, cols = x.shape
+    codes = torch.zeros((rows, cols), dtype=torch.float8_e4m3fn, device="cuda")
+    shape = (kb_of(cols), rows) if block_rows == 1 else (-(-rows // 128), kb_of(cols))
+    scales = torch.zeros(shape, device="cuda")
+    assert sp.quantize_fp8(None, x, codes, scales, block_rows) == 0
+    return codes, scales
+
+
+def check_quantized(x, codes, scales, block_rows):
+    want, want_scales = reference_codes(x.double().cpu().numpy(), block_rows)
+    got_scales = scales.cpu().numpy()
+    assert np.array_equal(got_scales.T if block_rows == 1 else got_scales, want_scales)
+    got = codes.float().double().cpu().numpy()
+    assert np.array_equal(got, want, equal_nan=True)
+    assert np.array_equal(np.signbit(got[~np.isnan(want)]), np.signbit(want[~np.isnan(want)]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("rows,cols", [(1, 16), (1, 9216), (7, 144), (8, 1024), (129, 400), (300, 2064), (1025, 1040)])
+def test_quantize(sp, rows, cols, block_rows, dtype):
+    g = rng(rows, cols)
+    x = torch.randn((rows, cols), device="cuda", generator=g) * torch.exp(2 * torch.randn((cols,), device="cuda", generator=g))
+    x[rows // 2, : cols // 2] = 0.0
+    x = x.to(dtype)
+    check_quantized(x, *quantize(sp, x, block_rows), block_rows)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+def test_quantize_borders(sp, dtype):
+    """Ties, their neighbours, the smallest codes, zeros of both signs, infinities, NaN, blocks of nothing, extreme blocks."""
+    mids = (E4M3[1:] + E4M3[:-1]) / 2
+    rows = []
+    for power in (0, -3, 4 if dtype is torch.float16 else 60):  # amax = 448 * 2^power: the scale is a power of two
+        t = torch.tensor(np.concatenate([mids, -mids, E4M3, [0.0, -0.0]]) * 2.0 ** power).to(dtype)
+        up, down = (t.view(torch.int16) + 1).view(dtype), (t.view(torch.int16) - 1).view(dtype)
+        for v in (t, up, down):
+            v = v[torch.isfinite(v) & (v.abs() <= 448.0 * 2.0 ** power)]
+            v = torch.cat([v, torch.zeros(-len(v) % 127, dtype=dtype)]).view(-1, 127)
+            rows.append(torch.cat([v, torch.full((len(v), 1), 448.0 * 2.0 ** power, dtype=dtype)], 1))
+    special = torch.zeros((9, 128), dtype=dtype)
+    special[0, 3] = float("inf")
+    special[0, 4] = 1.0
+    special[1, 100] = float("nan")
+    special[1, :50] = torch.linspace(-3, 3, 50).to(dtype)
+    special[2] = float("-inf")
+    special[3, 7] = torch.finfo(dtype).max
+    special[3, 8] = torch.finfo(dtype).tiny
+    special[4] = torch.finfo(dtype).smallest_normal / 4
+    special[5, 0] = torch.finfo(dtype).max
+    special[5, 1:] = -torch.finfo(dtype).max
+    special[6, 64:] = -0.0
+    special[7, 1] = 2.0 ** -24
+    special[8, ::2] = 1.0 / 3
+    rows.append(special)
+    x = torch.cat(rows).cuda().contiguous()
+    check_quantized(x, *quantize(sp, x, 1), 1)
+    check_quantized(x[:, :].contiguous(), *quantize(sp, x, 128), 128)
+
+
+def test_quantize_every_fp16_value(sp):
+    """All finite halves under 32 different scales."""
+    values = torch.arange(0, 65536, dtype=torch.int32).to(torch.int16).view(torch.float16)
+    values = values[torch.isfinite(values)]
+    for step in range(32):
+        top = float(values.abs().max()) * (1.0 - step / 67.0)
+        v = values[values.abs() <= top]
+        v = torch.cat([v, torch.zeros(-len(v) % 127, dtype=v.dtype)]).view(-1, 127)
+        x = torch.cat([v, torch.full((len(v), 1), top, dtype=v.dtype)], 1).cuda()
+        check_quantized(x, *quantize(sp, x, 1), 1)
+
+
+def test_quantize_groups_of_weights(sp):
+    x = torch.randn((3, 200, 272), device="cuda", generator=rng(3)).to(torch.bfloat16)
+    codes, scales = torch.zeros(x.shape, dtype=torch.uint8, device="cuda"), torch.zeros((3, 2, 3), device="cuda")
+    assert sp.quantize_fp8(None, x, codes, scales, 128) == 0
+    for e in range(3):
+        check_quantized(x[e], codes[e].view(torch.float8_e4m3fn), scales[e], 128)
+
+
+# ---------------------------------------------------------------- as they are used
+def test_feed_forward_through_experts(sp):
+    """Tokens sorted by expert through two 8-bit layers with a ReLU between them, all on one stream, the group borders and
+    the second layer's operands written by the kernels just ahead.  Each stage against its definition on the stage's inputs."""
+    tokens, hidden, inner, groups = 45, 512, 1040, 6
+    g = rng(77)
+    x = torch.randn((tokens, hidden), device="cuda", generator=g).to(torch.bfloat16)
+    weights = [torch.randn(s, device="cuda", generator=g).mul_(0.05).to(torch.bfloat16) for s in ((groups, inner, hidden), (groups, hidden, inner))]
+    packed = []
+    for w in weights:
+        codes = torch.empty(w.shape, dtype=torch.float8_e4m3fn, device="cuda")
+        scales = torch.empty((groups, kb_of(w.shape[1]), kb_of(w.shape[2])), device="cuda")
+        assert sp.quantize_fp8(None, w, codes, scales, 128) == 0
+        packed.append((codes, scales))
+    expert = torch.randint(0, groups - 1, (tokens,), device="cuda", generator=g)
+    order = torch.argsort(expert, stable=True)
+    off = torch.searchsorted(expert[order].contiguous(), torch.arange(groups + 1, device="cuda")).to(torch.int32)
+    rows = x[order].contiguous()
+    for layer, (codes, scales) in enumerate(packed):
+        m, k = codes.shape[1:]
+        b, sb = quantize(sp, rows, 1)
+        c = torch.full((tokens, m), 7.0, dtype=torch.bfloat16, device="cuda")
+        assert sp.grouped_fp8_linear(None, codes, scales, b, sb, c, off, groups, m, tokens, k, workspace_for(sp, groups, m, tokens, k, True)) == 0
+        av = codes.double() * scales.double().repeat_interleave(128, 1)[:, :m].repeat_interleave(128, 2)[:, :, :k]
+        bv = b.double() * sb.double().t().repeat_interleave(128, 1)[:, :k]
+        check(c, av, bv, off.tolist(), k, torch.bfloat16)
+        check_quantized(rows, b, sb, 1)
+        rows = torch.relu(c)
+    assert sp.device_status() == 0
+
+
+def test_python_refusals(sp):
+    m, n, k = 128, 4, 128
+    a, sa, b, sb, _, _ = random_operands(1, m, n, k, None, 1)
+    c = torch.zeros((n, m), dtype=torch.float16, device="cuda")
+    off = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    ok = dict(A=a, A_scales=sa, B=b, B_scales=sb, C=c)
+    for name, bad in [("A", a.float()), ("A", a.cpu()), ("A", a[:, :64]), ("B", b.t()), ("B", b[:3]), ("A_scales", sa.half()), ("B_scales", sb[:, :3]),
+                      ("C", c.float()), ("C", torch.zeros((m, n), dtype=torch.float16, device="cuda").t()), ("C", c[:3])]:
+        with pytest.raises(ValueError):
+            t = dict(ok, **{name: bad})
+            sp.fp8_linear(None, t["A"], t["A_scales"], t["B"], t["B_scales"], t["C"], m, n, k, None)
+    with pytest.raises(ValueError):
+        sp.grouped_linear(None, a.half(), b.bfloat16(), c, off, 1, m, n, k, None)
+    with pytest.raises(ValueError):
+        sp.grouped_fp8_linear(None, a, sa, b, sb, c, off.long(), 1, m, n, k, None)
+    with pytest.raises(ValueError):
+        sp.grouped_fp8_linear(None, a, sa, b, sb, c, off, 2, m, n, k, None)
+    with pytest.raises(ValueError):
+        sp.quantize_fp8(None, c, b, sb, 2)
+    with pytest.raises(ValueError):
+        sp.quantize_fp8(None, c.float(), b, sb, 1)
+    assert sp.fp8_linear(None, a[:, :120].contiguous(), sa, b[:, :120].contiguous(), sb, c, m, n, 120, None) == 1
+    small = torch.zeros(64, dtype=torch.uint8, device="cuda")  # too small a workspace is not used
+    assert sp.fp8_linear(None, a, sa, b, sb, c, m, n, k, small) == 0
+    assert not bool(small.any())
