@@ -125,8 +125,8 @@ cudaError_t launch(cudaStream_t stream, LinearParams& p, const LinearShape& s)
         }
         sms = d.sm_count;
     }
-    const int stage_bytes = kLinearBoxBytes + s.nt * 128;
-    const int fixed       = kLinearFixedSmem + (EIGHT ? kScaleSlots * 128 * 4 : 0) + s.groups * 12;
+    const int stage_bytes = kStepBlocks * (kLinearBoxBytes + s.nt * 128);
+    const int fixed       = kLinearFixedSmem + (EIGHT ? 2 * kGroupScales * 4 : 0) + s.groups * 12;
     p.stages              = std::min(kLinearMaxStages, (kMaxDynamicSmem - fixed) / stage_bytes);
 
     cudaLaunchConfig_t config = {};
@@ -175,6 +175,7 @@ cudaError_t linear(cudaStream_t stream, LinearShape s, const void* A, const floa
     p.m        = s.m;
     p.n        = s.n;
     p.kb       = s.kb;
+    p.steps    = (s.kb - 1) / kStepBlocks + 1;
     p.nt       = s.nt;
     p.b_box    = s.b_box;
     p.bf16     = C_type == SPMM_B200_BF16;
@@ -182,7 +183,7 @@ cudaError_t linear(cudaStream_t stream, LinearShape s, const void* A, const floa
     if (workspace && workspace_bytes >= workspace_needed(s)) {
         p.counters = static_cast<unsigned*>(workspace);
         p.slots    = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
-        p.overhead = 4;
+        p.overhead = 2;
     }
     return s.eight ? launch<true>(stream, p, s) : launch<false>(stream, p, s);
 }

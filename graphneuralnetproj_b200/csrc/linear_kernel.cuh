@@ -7,12 +7,15 @@
 // A block takes 128 rows of A as the M side of tcgen05.mma and up to 128 tokens as its N side (N is a run-time field of
 // the instruction descriptor, so a group's last few tokens cost no more than they must), because weights are what there
 // is always plenty of: one token still fills the tensor core's 128 lanes and streams A at full rate.  A k-block is 128
-// bytes of K (64 halves or 128 codes, i.e. one scale block): one 128-byte-swizzled TMA box of A and one or a few of B
-// per ring stage, four MMAs.
+// bytes of K (64 halves or 128 codes, i.e. one scale block), the width of a 128-byte-swizzled TMA box; a ring stage
+// holds a step of two k-blocks, because the MMA lane's waits and commits cost a few hundred cycles per stage.
 //
 // fp16 / bf16 accumulate the whole K range in TMEM.  With scales every k-block is a product of its own: the MMA warp
-// writes it to one of four TMEM buffers in turn, and the epilogue warps add it to fp32 registers, each column times
-// (token's scale) * (block's scale), while the tensor core is at the next ones.
+// fills one half of TMEM with the products of a group of one to four steps (as many as fit side by side), and the
+// epilogue warps add them to fp32 registers, each column times (token's scale) * (block's scale), while the tensor core
+// fills the other half.  One hand-over per group, not per step: with a wait for the product and another for the scales
+// in every step, the few hundred instructions of the epilogue warps around them took 1.4 us per step, twice what the
+// 32 KB of a step take to arrive (36864 x 9216, 16 tokens: 104 us, against 70 without the second wait).
 //
 // Roles: warp 0 TMA, warp 1 MMA issue and TMEM, warp 2 scales, warps 4..11 epilogue (warp % 4 = quarter of the TMEM
 // lanes, warp / 4 - 1 = every other chunk of columns).  Every wait is bounded; a block that gives up records it.
@@ -36,7 +39,9 @@ constexpr int kLinearMaxStages = 12;
 constexpr int kLinearMaxGroups = 1024;
 constexpr int kLinearRows      = 128;                // lanes of a block's tile
 constexpr int kLinearBoxBytes  = kLinearRows * 128;  // its operand, one k-block
-constexpr int kScaleSlots      = 8;
+constexpr int kStepBlocks      = 2;  // k-blocks per ring stage
+constexpr int kGroupBlocks     = 8;  // k-blocks of a group at most
+constexpr int kGroupScales     = 256;  // scales of a group: k-blocks x columns
 constexpr int kEpilogueTeams   = 8;  // epilogue warps
 constexpr int kPieceCounters   = 4096;  // arrival counters at the head of a workspace
 constexpr int kLinearFixedSmem = 1024 /* alignment */ + 512 /* barriers */;
@@ -49,7 +54,9 @@ struct LinearParams {
     const int*   offsets;  // [groups + 1], or null: one group of all N tokens
     unsigned*    counters;
     float*       slots;
-    int          groups, m, n, kb;
+    int          groups, m, n;
+    int          kb;        // k-blocks
+    int          steps;     // pairs of them
     int          nt;        // tokens per tile at most
     int          b_box;     // tokens per TMA box
     int          stages;
@@ -62,39 +69,61 @@ struct LinearTile {
     int group, m0, row0, rows;  // first row of A, first token, tokens
 };
 
-// One warp waits: lane 0 polls, the others follow.
-__device__ __forceinline__ bool linear_warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_word, int lane)
+// Steps whose products fit side by side into 256 TMEM columns, and the columns of each.
+SPMM_B200_HD int linear_group_steps(int nt)
 {
-    int ok = 1;
-    if (lane == 0)
-        ok = ptx::mbar_wait_bounded(bar, parity, abort_word);
-    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+    return nt <= 32 ? 4 : (nt <= 64 ? 2 : 1);
+}
+
+// A bounded wait of all lanes of a warp, or of one.  Parked at once: here most waits are long, and the polling of ten warps
+// slows the others down (64 experts of 2048 x 4096 in bf16: 130 us with 64 polls before parking, 121 without).
+__device__ __forceinline__ bool linear_wait(uint32_t bar, uint32_t parity, volatile int* abort_word)
+{
+    uint64_t start = 0;
+#pragma unroll 1
+    for (uint32_t polls = 0;; polls++) {
+        if (ptx::mbar_try_wait_suspend(bar, parity, ptx::kSuspendNs))
+            return true;
+        if (*abort_word != 0)
+            return false;
+        if ((polls & 255u) == 0) {
+            const uint64_t now = ptx::global_timer_ns();
+            if (start == 0)
+                start = now;
+            else if (now - start > ptx::kWaitLimitNs) {
+                *abort_word = 1;
+                return false;
+            }
+        }
+    }
 }
 
 template<bool EIGHT>
 __global__ void __launch_bounds__(kLinearThreads, 1)
 linear_kernel(const __grid_constant__ LinearParams p)
 {
-    constexpr int NMAX = 128;             // columns of a TMEM buffer
-    constexpr int NBUF = 512 / NMAX;      // TMEM buffers
+    constexpr int NMAX = 128;             // columns of a tile at most
+    constexpr int BUFS = 2;               // halves of TMEM
     constexpr int CH   = 16;              // columns per chunk
     constexpr int NCH  = NMAX / (2 * CH); // chunks per epilogue warp
 
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base   = (ptx::smem_addr(smem_raw) + 1023u) & ~1023u;
     uint8_t*       smem        = smem_raw + (smem_base - ptx::smem_addr(smem_raw));
-    const uint32_t stage_bytes = kLinearBoxBytes + p.nt * 128u;
+    const uint32_t part_bytes  = p.nt * 128u;  // B's part of a k-block
+    const uint32_t stage_bytes = kStepBlocks * (kLinearBoxBytes + part_bytes);
+    const int      group_steps = linear_group_steps(p.nt);
+    const int      acc_shift   = p.nt <= 32 ? 5 : (p.nt <= 64 ? 6 : 7);
+    const int      acc_width   = 1 << acc_shift;  // TMEM columns of a product: group_steps * kStepBlocks * acc_width = 256
     const uint32_t scale_off   = p.stages * stage_bytes;
-    const uint32_t bar_off     = scale_off + (EIGHT ? kScaleSlots * NMAX * 4u : 0u);
+    const uint32_t bar_off     = scale_off + (EIGHT ? BUFS * kGroupScales * 4u : 0u);
     const uint32_t bar_base    = smem_base + bar_off;
     float* const   scale_ring  = reinterpret_cast<float*>(smem + scale_off);
     auto full       = [&](int s) { return bar_base + 8u * s; };
     auto empty      = [&](int s) { return bar_base + 8u * (kLinearMaxStages + s); };
     auto acc_full   = [&](int b) { return bar_base + 8u * (2 * kLinearMaxStages + b); };
-    auto acc_free   = [&](int b) { return bar_base + 8u * (2 * kLinearMaxStages + NBUF + b); };
-    auto scale_full = [&](int s) { return bar_base + 8u * (2 * kLinearMaxStages + 2 * NBUF + s); };
-    auto scale_free = [&](int s) { return bar_base + 8u * (2 * kLinearMaxStages + 2 * NBUF + kScaleSlots + s); };
-    constexpr uint32_t kWords = 8u * (2 * kLinearMaxStages + 2 * NBUF + 2 * kScaleSlots);
+    auto acc_free   = [&](int b) { return bar_base + 8u * (2 * kLinearMaxStages + BUFS + b); };
+    constexpr uint32_t kWords = 8u * (2 * kLinearMaxStages + 2 * BUFS);
     static_assert(kWords + 64 <= 512, "barrier block");
     volatile uint32_t* tmem_slot  = reinterpret_cast<volatile uint32_t*>(smem + bar_off + kWords);
     volatile int*      abort_word = reinterpret_cast<volatile int*>(smem + bar_off + kWords + 4);
@@ -110,13 +139,9 @@ linear_kernel(const __grid_constant__ LinearParams p)
             ptx::mbar_init(full(s), 1);
             ptx::mbar_init(empty(s), 1);
         }
-        for (int b = 0; b < NBUF; b++) {
-            ptx::mbar_init(acc_full(b), 1);
+        for (int b = 0; b < BUFS; b++) {
+            ptx::mbar_init(acc_full(b), EIGHT ? 2 : 1);  // the products, and the scales
             ptx::mbar_init(acc_free(b), kEpilogueTeams);
-        }
-        for (int s = 0; s < kScaleSlots; s++) {
-            ptx::mbar_init(scale_full(s), 1);
-            ptx::mbar_init(scale_free(s), kEpilogueTeams);
         }
         *abort_word = 0;
         ptx::mbar_init_fence();
@@ -165,7 +190,7 @@ linear_kernel(const __grid_constant__ LinearParams p)
         ptx::tc_fence_after_sync();
     }
     const uint32_t        tmem_base = *tmem_slot;
-    const LinearPartition part      = make_linear_partition(tile_end[p.groups - 1], p.kb, static_cast<int>(gridDim.x), p.overhead);
+    const LinearPartition part      = make_linear_partition(tile_end[p.groups - 1], p.steps, static_cast<int>(gridDim.x), p.overhead);
     const int             worker    = static_cast<int>(blockIdx.x);
 
     auto locate = [&](int tile) {
@@ -193,30 +218,36 @@ linear_kernel(const __grid_constant__ LinearParams p)
     if (warp == 0) {
         // ------------------------------------------------------------ TMA
         if (lane == 0) {
-            bool ok = true;
-            int  s  = 0;
+            bool     ok = true;
+            int      s  = 0;
+            uint32_t phase = 1;  // of the stages' "empty" barriers: the first round finds them so
             for (int i = 0; ok; i++) {
                 const LinearSegment seg = linear_segment(part, worker, i);
                 if (seg.tile < 0)
                     break;
                 const LinearTile t     = locate(seg.tile);
                 const int        boxes = (columns(t) + p.b_box - 1) / p.b_box;
-                const uint32_t   bytes = kLinearBoxBytes + boxes * p.b_box * 128u;
+                const uint32_t   bytes = kStepBlocks * (kLinearBoxBytes + boxes * p.b_box * 128u);
 #pragma unroll 1
                 for (int k = seg.kb0; k < seg.kb1; k++) {
-                    if (issued >= p.stages) {
-                        ok = ptx::mbar_wait_bounded(empty(s), ((issued / p.stages) - 1) & 1, abort_word);
-                        if (!ok)
-                            break;
-                    }
+                    ok = linear_wait(empty(s), phase, abort_word);
+                    if (!ok)
+                        break;
                     const uint32_t dst = smem_base + s * stage_bytes;
                     ptx::mbar_arrive_expect_tx(full(s), bytes);
-                    ptx::tma_load_3d(dst, &p.a_map, k * 128, t.m0, t.group, full(s));
-                    for (int b = 0; b < boxes; b++)
-                        ptx::tma_load_3d(dst + kLinearBoxBytes + b * p.b_box * 128, &p.b_map, k * 128, t.row0 + b * p.b_box, 0, full(s));
+#pragma unroll
+                    for (int h = 0; h < kStepBlocks; h++) {
+                        const int x = (k * kStepBlocks + h) * 128;  // a k-block behind the end of K arrives as zeros
+                        ptx::tma_load_3d(dst + h * kLinearBoxBytes, &p.a_map, x, t.m0, t.group, full(s));
+                        for (int b = 0; b < boxes; b++)
+                            ptx::tma_load_3d(dst + kStepBlocks * kLinearBoxBytes + h * part_bytes + b * p.b_box * 128, &p.b_map, x,
+                                             t.row0 + b * p.b_box, 0, full(s));
+                    }
                     issued++;
-                    if (++s == p.stages)
+                    if (++s == p.stages) {
                         s = 0;
+                        phase ^= 1;
+                    }
                 }
             }
         }
@@ -224,8 +255,9 @@ linear_kernel(const __grid_constant__ LinearParams p)
     else if (warp == 1) {
         // ------------------------------------------------------------ MMA
         if (lane == 0) {
-            bool ok  = true;
-            int  use = 0, s = 0, phase = 0;  // use: TMEM buffers handed out
+            bool           ok  = true;
+            int            s   = 0;
+            uint32_t       phase = 0, use = 0;  // use: halves of TMEM handed over
             const uint64_t a_desc0 = ptx::make_smem_desc(smem_base, 16, 1024, ptx::kSwizzle128B);
             for (int i = 0; ok; i++) {
                 const LinearSegment seg = linear_segment(part, worker, i);
@@ -233,31 +265,40 @@ linear_kernel(const __grid_constant__ LinearParams p)
                     break;
                 const uint32_t idesc =
                     ptx::make_idesc_f16_f32(kLinearRows, columns(locate(seg.tile)), false, false) | (!EIGHT && p.bf16 ? ptx::kIdescBf16 : 0u);
+                int      left   = 0;  // steps that the current half still takes
+                uint32_t d_tmem = 0;
 #pragma unroll 1
                 for (int k = seg.kb0; k < seg.kb1; k++) {
-                    const uint32_t d_tmem = tmem_base + (use % NBUF) * NMAX;
-                    const bool     fresh  = EIGHT || k == seg.kb0;
-                    if (fresh && use >= NBUF && !ptx::mbar_wait_bounded(acc_free(use % NBUF), (use / NBUF - 1) & 1, abort_word)) {
-                        ok = false;
-                        break;
+                    const bool fresh = left == 0;
+                    if (fresh) {
+                        left = EIGHT ? min(group_steps, seg.kb1 - k) : seg.kb1 - k;
+                        ok   = linear_wait(acc_free(use & 1), ((use >> 1) & 1) ^ 1, abort_word);
+                        if (!ok)
+                            break;
                     }
-                    if (!ptx::mbar_wait_bounded(full(s), phase, abort_word)) {
-                        ok = false;
+                    ok = linear_wait(full(s), phase, abort_word);
+                    if (!ok)
                         break;
-                    }
                     ptx::tc_fence_after_sync();
+                    if (fresh)
+                        d_tmem = tmem_base + (use & 1) * kGroupScales;
                     const uint64_t a_desc = a_desc0 + static_cast<uint64_t>((s * stage_bytes) >> 4);
-                    const uint64_t b_desc = a_desc + (kLinearBoxBytes >> 4);
+                    const uint64_t b_desc = a_desc + (kStepBlocks * kLinearBoxBytes >> 4);
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        if (EIGHT)
-                            ptx::umma_f8_ss(d_tmem, a_desc + j * 2, b_desc + j * 2, idesc, j > 0);
-                        else
-                            ptx::umma_f16_ss(d_tmem, a_desc + j * 2, b_desc + j * 2, idesc, !fresh || j > 0);
-                    }
+                    for (int h = 0; h < kStepBlocks; h++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const uint64_t a = a_desc + h * (kLinearBoxBytes >> 4) + j * 2, b = b_desc + h * (part_bytes >> 4) + j * 2;
+                            if (EIGHT)
+                                ptx::umma_f8_ss(d_tmem + h * acc_width, a, b, idesc, j > 0);
+                            else
+                                ptx::umma_f16_ss(d_tmem, a, b, idesc, !fresh || h > 0 || j > 0);
+                        }
                     ptx::umma_commit(empty(s));
-                    if (EIGHT || k == seg.kb1 - 1) {
-                        ptx::umma_commit(acc_full(use % NBUF));
+                    if (EIGHT)
+                        d_tmem += kStepBlocks * acc_width;
+                    if (--left == 0) {
+                        ptx::umma_commit(acc_full(use & 1));
                         use++;
                     }
                     if (++s == p.stages) {
@@ -271,57 +312,64 @@ linear_kernel(const __grid_constant__ LinearParams p)
     else if (warp == 2) {
         // ------------------------------------------------------------ scales
         if (EIGHT) {
-            constexpr int PER = NMAX / 32, BATCH = 4;
-            const int     blocks_m = tiles_m;
-            int           use      = 0;
-            bool          ok       = true;
-            for (int i = 0; ok; i++) {
-                const LinearSegment seg = linear_segment(part, worker, i);
-                if (seg.tile < 0)
-                    break;
-                const LinearTile t  = locate(seg.tile);
-                const float*     sa = p.a_scales + (static_cast<size_t>(t.group) * blocks_m + t.m0 / kLinearRows) * p.kb;
-                const float*     sb = p.b_scales + t.row0;
-                float            a[BATCH], b[BATCH][PER];
-                auto fetch = [&](int k0) {
+            // A group's scales are loaded two groups ahead: with the memory system busy a load takes as long as several
+            // steps.  Value v of a group is k-block v / acc_width, column v % acc_width; lane l has v = l, l + 32, ...
+            constexpr int PER = kGroupScales / 32;
+            struct Ahead {
+                float a, b[PER];
+            };
+            int           next_i = 0, next_k = 0;  // the segment and step that `fetch` is at
+            LinearSegment next_seg = linear_segment(part, worker, 0);
+            LinearTile    next_tile{};
+            if (next_seg.tile >= 0) {
+                next_tile = locate(next_seg.tile);
+                next_k    = next_seg.kb0;
+            }
+            auto fetch = [&](Ahead& f) {  // false: no groups left
+                if (next_seg.tile < 0)
+                    return false;
+                const float* sa = p.a_scales + (static_cast<size_t>(next_tile.group) * tiles_m + next_tile.m0 / kLinearRows) * p.kb;
+                const int    k0 = next_k * kStepBlocks;
+                f.a             = __ldg(sa + min(k0 + (lane & (kGroupBlocks - 1)), p.kb - 1));
 #pragma unroll
-                    for (int u = 0; u < BATCH; u++) {
-                        const int k = min(k0 + u, seg.kb1 - 1);
-                        a[u]        = __ldg(sa + k);
-#pragma unroll
-                        for (int j = 0; j < PER; j++)
-                            b[u][j] = lane + 32 * j < t.rows ? __ldg(sb + static_cast<size_t>(k) * p.n + lane + 32 * j) : 0.0f;
-                    }
-                };
-                fetch(seg.kb0);
-#pragma unroll 1
-                for (int k0 = seg.kb0; k0 < seg.kb1 && ok; k0 += BATCH) {
-                    float v[BATCH][PER];
-#pragma unroll
-                    for (int u = 0; u < BATCH; u++)
-#pragma unroll
-                        for (int j = 0; j < PER; j++)
-                            v[u][j] = a[u] * b[u][j];
-                    if (k0 + BATCH < seg.kb1)
-                        fetch(k0 + BATCH);
-#pragma unroll
-                    for (int u = 0; u < BATCH; u++) {
-                        if (k0 + u < seg.kb1 && ok) {
-                            const int slot = use % kScaleSlots;
-                            if (use >= kScaleSlots)
-                                ok = linear_warp_wait(scale_free(slot), (use / kScaleSlots - 1) & 1, abort_word, lane);
-                            if (ok) {
-#pragma unroll
-                                for (int j = 0; j < PER; j++)
-                                    scale_ring[slot * NMAX + lane + 32 * j] = v[u][j];
-                                __syncwarp();
-                                if (lane == 0)
-                                    ptx::mbar_arrive(scale_full(slot));
-                                use++;
-                            }
-                        }
+                for (int j = 0; j < PER; j++) {
+                    const int v = lane + 32 * j, block = min(k0 + (v >> acc_shift), p.kb - 1), column = v & (acc_width - 1);
+                    f.b[j] = __ldg(p.b_scales + static_cast<size_t>(block) * p.n + next_tile.row0 + min(column, next_tile.rows - 1));
+                }
+                next_k += group_steps;
+                if (next_k >= next_seg.kb1) {
+                    next_seg = linear_segment(part, worker, ++next_i);
+                    if (next_seg.tile >= 0) {
+                        next_tile = locate(next_seg.tile);
+                        next_k    = next_seg.kb0;
                     }
                 }
+                return true;
+            };
+            Ahead    one, two;
+            uint32_t use = 0;
+            auto     lay_out = [&](const Ahead& f) {
+                if (!linear_wait(acc_free(use & 1), ((use >> 1) & 1) ^ 1, abort_word))
+                    return false;
+#pragma unroll
+                for (int j = 0; j < PER; j++) {
+                    const int v = lane + 32 * j;
+                    scale_ring[(use & 1) * kGroupScales + v] = f.b[j] * __shfl_sync(0xffffffffu, f.a, v >> acc_shift);
+                }
+                __syncwarp();
+                if (lane == 0)
+                    ptx::mbar_arrive(acc_full(use & 1));
+                use++;
+                return true;
+            };
+            bool have_one = fetch(one), have_two = fetch(two);
+            while (have_one) {
+                if (!lay_out(one))
+                    break;
+                have_one = fetch(one);
+                if (!have_two || !lay_out(two))
+                    break;
+                have_two = fetch(two);
             }
         }
     }
@@ -331,7 +379,7 @@ linear_kernel(const __grid_constant__ LinearParams p)
         const int      row     = (warp & 3) * 32 + lane;  // lane of the accumulator
         const uint32_t tmem_at = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         auto           col_of  = [&](int i) { return (2 * i + team) * CH; };
-        int            use     = 0;
+        uint32_t       use     = 0;
         bool           ok      = true;
         for (int i = 0; ok; i++) {
             const LinearSegment seg = linear_segment(part, worker, i);
@@ -340,58 +388,61 @@ linear_kernel(const __grid_constant__ LinearParams p)
             const LinearTile t = locate(seg.tile);
             const int        n = columns(t);
             float            acc[EIGHT ? NCH * CH : 1];
-            uint32_t         chunk[CH];
             if (EIGHT) {
 #pragma unroll
                 for (int c = 0; c < NCH * CH; c++)
                     acc[c] = 0.0f;
 #pragma unroll 1
-                for (int k = seg.kb0; k < seg.kb1; k++, use++) {
-                    const int slot = use % kScaleSlots, buf = use % NBUF;
-                    ok = linear_warp_wait(scale_full(slot), (use / kScaleSlots) & 1, abort_word, lane)
-                         && linear_warp_wait(acc_full(buf), (use / NBUF) & 1, abort_word, lane);
+                for (int k = seg.kb0; k < seg.kb1; k += group_steps, use++) {
+                    ok = linear_wait(acc_full(use & 1), (use >> 1) & 1, abort_word);
                     if (!ok)
                         break;
                     ptx::tc_fence_after_sync();
+                    const int    blocks  = min(group_steps, seg.kb1 - k) * kStepBlocks;
+                    uint32_t     from    = tmem_at + (use & 1) * kGroupScales;
+                    const float* scales  = scale_ring + (use & 1) * kGroupScales;
+#pragma unroll 1
+                    for (int h = 0; h < blocks; h++, from += acc_width, scales += acc_width) {
 #pragma unroll
-                    for (int c = 0; c < NCH; c++) {
-                        if (col_of(c) < n) {
-                            ptx::tmem_ld_x16(tmem_at + buf * NMAX + col_of(c), chunk);
-                            ptx::tmem_ld_wait();
-                            const float4* sc = reinterpret_cast<const float4*>(scale_ring + slot * NMAX + col_of(c));
+                        for (int c = 0; c < NCH; c++) {
+                            if (col_of(c) < n) {
+                                uint32_t product[CH];
+                                ptx::tmem_ld_x16(from + col_of(c), product);
+                                ptx::tmem_ld_wait();
+                                const float4* sc = reinterpret_cast<const float4*>(scales + col_of(c));
 #pragma unroll
-                            for (int j = 0; j < CH / 4; j++) {
-                                const float4 f = sc[j];
-                                acc[c * CH + 4 * j] += __uint_as_float(chunk[4 * j]) * f.x;
-                                acc[c * CH + 4 * j + 1] += __uint_as_float(chunk[4 * j + 1]) * f.y;
-                                acc[c * CH + 4 * j + 2] += __uint_as_float(chunk[4 * j + 2]) * f.z;
-                                acc[c * CH + 4 * j + 3] += __uint_as_float(chunk[4 * j + 3]) * f.w;
+                                for (int j = 0; j < CH / 4; j++) {
+                                    const float4 f = sc[j];
+                                    acc[c * CH + 4 * j] += __uint_as_float(product[4 * j]) * f.x;
+                                    acc[c * CH + 4 * j + 1] += __uint_as_float(product[4 * j + 1]) * f.y;
+                                    acc[c * CH + 4 * j + 2] += __uint_as_float(product[4 * j + 2]) * f.z;
+                                    acc[c * CH + 4 * j + 3] += __uint_as_float(product[4 * j + 3]) * f.w;
+                                }
                             }
                         }
                     }
                     ptx::tc_fence_before_sync();
                     __syncwarp();
-                    if (lane == 0) {
-                        ptx::mbar_arrive(acc_free(buf));
-                        ptx::mbar_arrive(scale_free(slot));
-                    }
+                    if (lane == 0)
+                        ptx::mbar_arrive(acc_free(use & 1));
                 }
             }
             else {
-                ok = linear_warp_wait(acc_full(use % NBUF), (use / NBUF) & 1, abort_word, lane);
+                ok = linear_wait(acc_full(use & 1), (use >> 1) & 1, abort_word);
                 ptx::tc_fence_after_sync();
             }
             if (!ok)
                 break;
             // chunk c of this warp as fp32: out of the registers, or out of TMEM
             auto values = [&](int c, float* v) {
-                if (EIGHT) {
+                if constexpr (EIGHT) {
 #pragma unroll
                     for (int j = 0; j < CH; j++)
                         v[j] = acc[c * CH + j];
                 }
                 else {
-                    ptx::tmem_ld_x16(tmem_at + (use % NBUF) * NMAX + col_of(c), chunk);
+                    uint32_t chunk[CH];
+                    ptx::tmem_ld_x16(tmem_at + (use & 1) * kGroupScales + col_of(c), chunk);
                     ptx::tmem_ld_wait();
 #pragma unroll
                     for (int j = 0; j < CH; j++)
@@ -475,7 +526,7 @@ linear_kernel(const __grid_constant__ LinearParams p)
                 ptx::tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0)
-                    ptx::mbar_arrive(acc_free(use % NBUF));
+                    ptx::mbar_arrive(acc_free(use & 1));
                 use++;
             }
         }

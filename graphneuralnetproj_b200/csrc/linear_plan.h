@@ -1,6 +1,7 @@
 // How the tiles of a linear layer are shared out between thread blocks (linear_kernel.cuh).
 //
-// The product is a list of output tiles, each `kb` k-blocks deep (128 bytes of K per k-block).  `workers` blocks (or
+// The product is a list of output tiles, each `kb` k-blocks deep (a k-block here is
+// one ring stage of the kernel).  `workers` blocks (or
 // pairs of blocks) run at the same time, one per SM (pair of SMs).  Tiles are dealt out whole, worker c taking tiles
 // c, c + workers, ...; what does not fill a last round -- or everything, where there are fewer tiles than workers, as
 // for a few tokens -- can instead be cut into equal runs of k-blocks, one run per worker.  A run then covers the end of
@@ -36,7 +37,7 @@ struct LinearSegment {
 };
 
 constexpr int kMaxPieces = 16;  // pieces of one tile: bounds what the last worker has to add up
-constexpr int kMinRun    = 4;   // k-blocks a run has at least
+constexpr int kMinRun    = 2;   // k-blocks a run has at least
 
 // overhead: what parking and adding a piece costs, in k-blocks; < 0: no workspace, nothing is cut
 SPMM_B200_HD LinearPartition make_linear_partition(int tiles, int kb, int workers, int overhead)
