@@ -6,6 +6,7 @@
 #include "../../include/spmm_b200.h"
 #include "linear_api.h"
 #include "linear_kernel.cuh"
+#include "linear_pair_kernel.cuh"
 
 namespace spmm_b200 {
 namespace {
@@ -20,9 +21,10 @@ struct LinearShape {
     bool ragged;  // group borders are read on the device
 
     // What follows from the sizes:
-    int    kb;
-    int    nt, b_box;
-    size_t slot_bytes;
+    bool   pair;        // tiles of 256 x 256 on pairs of SMs
+    int    kb;          // k-blocks
+    int    nt, b_box;   // tokens per tile, and per TMA box
+    size_t slot_bytes;  // a worker's piece of a tile
 };
 
 bool aligned16(const void* p)
@@ -30,11 +32,20 @@ bool aligned16(const void* p)
     return (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
 }
 
-// Tokens per tile.  One matrix: as few tiles as 128 columns allow, of equal width.  Groups, whose sizes the host does
-// not know: twice the average, so that most groups are one tile and its ring stages are not mostly unused.
+// Which kernel, and tokens per tile.  One block per tile takes 128 tokens at most: one matrix is cut into as few tiles of
+// equal width as that allows; groups, whose sizes the host does not know, into tiles of twice the average, so that most
+// groups are one tile and its ring stages are not mostly unused.
 void choose_tiles(LinearShape& s)
 {
-    s.kb = (s.k * (s.eight ? 1 : 2) - 1) / 128 + 1;
+    s.kb            = (s.k * (s.eight ? 1 : 2) - 1) / 128 + 1;
+    const int group = s.ragged ? s.n / s.groups : s.n;  // tokens, on average
+    s.pair          = group > 128;
+    if (s.pair) {
+        s.nt         = kPairTile;
+        s.b_box      = s.eight ? kLinearRows : 64;
+        s.slot_bytes = 2 * static_cast<size_t>(kLinearRows) * kPairTile * sizeof(float);
+        return;
+    }
     if (!s.ragged) {
         const int tiles = std::max(1, (s.n - 1) / 128 + 1);
         s.nt            = std::max(16, ((s.n - 1) / tiles + 1 + 15) / 16 * 16);
@@ -48,9 +59,14 @@ void choose_tiles(LinearShape& s)
     s.slot_bytes = static_cast<size_t>(kLinearRows) * s.nt * sizeof(float);
 }
 
+int max_workers(const LinearShape& s)
+{
+    return s.pair ? kMaxWorkers / 2 : kMaxWorkers;
+}
+
 size_t workspace_needed(const LinearShape& s)
 {
-    return kCounterBytes + 2 * static_cast<size_t>(kMaxWorkers) * s.slot_bytes;
+    return kCounterBytes + 2 * static_cast<size_t>(max_workers(s)) * s.slot_bytes;
 }
 
 // Sizes that the format and the index arithmetic can describe.
@@ -91,55 +107,70 @@ cudaError_t describe(CUtensorMap& map, const void* base, long row_bytes, long ro
                : cudaErrorInvalidValue;
 }
 
+// What is looked up once per device and kernel: the blocks (or pairs) that run at the same time.
 struct LinearDevice {
-    int  sm_count     = 0;
-    bool attrs_set[2] = {};
+    int workers[4] = {};
 };
 
-template<bool EIGHT>
+template<bool EIGHT, bool PAIR>
 cudaError_t launch(cudaStream_t stream, LinearParams& p, const LinearShape& s)
 {
     int         device = 0;
     cudaError_t e      = cudaGetDevice(&device);
     if (e != cudaSuccess)
         return e;
-    static LinearDevice devices[64];
-    static std::mutex   lock;
-    auto                kern = linear_kernel<EIGHT>;
-    int                 sms  = 0;
-    {
-        std::lock_guard<std::mutex> guard(lock);
-        LinearDevice& d = devices[device & 63];
-        if (d.sm_count == 0) {
-            e = cudaDeviceGetAttribute(&d.sm_count, cudaDevAttrMultiProcessorCount, device);
-            if (e != cudaSuccess)
-                return e;
-        }
-        if (!d.attrs_set[EIGHT]) {
-            e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxDynamicSmem);
-            if (e != cudaSuccess) {
-                (void)cudaGetLastError();
-                return e;
-            }
-            d.attrs_set[EIGHT] = true;
-        }
-        sms = d.sm_count;
-    }
-    const int stage_bytes = kStepBlocks * (kLinearBoxBytes + s.nt * 128);
-    const int fixed       = kLinearFixedSmem + (EIGHT ? 2 * kGroupScales * 4 : 0) + s.groups * 12;
-    p.stages              = std::min(kLinearMaxStages, (kMaxDynamicSmem - fixed) / stage_bytes);
+    auto      kern        = PAIR ? linear_pair_kernel<EIGHT> : linear_kernel<EIGHT>;
+    const int stage_bytes = PAIR ? kPairStageBytes : kStepBlocks * (kLinearBoxBytes + s.nt * 128);
+    const int fixed       = kLinearFixedSmem + (EIGHT && !PAIR ? 2 * kGroupScales * 4 : 0) + s.groups * 12;
+    p.stages              = std::min(PAIR ? kPairStages : kLinearMaxStages, (kMaxDynamicSmem - fixed) / stage_bytes);
+    p.steps               = PAIR ? s.kb : (s.kb - 1) / kStepBlocks + 1;
 
     cudaLaunchConfig_t config = {};
-    config.gridDim            = dim3(std::min(sms, kMaxWorkers));
     config.blockDim           = dim3(kLinearThreads);
     config.dynamicSmemBytes   = fixed + p.stages * stage_bytes;
     config.stream             = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id                                         = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x                           = 2;
+    attr[1].val.clusterDim.y                           = 1;
+    attr[1].val.clusterDim.z                           = 1;
     config.attrs                                       = attr;
-    config.numAttrs                                    = 1;
-    e = cudaLaunchKernelEx(&config, kern, p);
+    config.numAttrs                                    = PAIR ? 2 : 1;
+
+    static LinearDevice devices[64];
+    static std::mutex   lock;
+    int                 workers = 0;
+    {
+        std::lock_guard<std::mutex> guard(lock);
+        int& known = devices[device & 63].workers[2 * PAIR + EIGHT];
+        if (known == 0) {
+            int sms = 0, found = 0;
+            e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+            if (e == cudaSuccess)
+                e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxDynamicSmem);
+            if (e == cudaSuccess && PAIR) {
+                cudaLaunchConfig_t probe = config;
+                probe.gridDim            = dim3(sms / 2 * 2);
+                probe.dynamicSmemBytes   = kMaxDynamicSmem;
+                probe.attrs              = attr + 1;
+                probe.numAttrs           = 1;
+                e                        = cudaOccupancyMaxActiveClusters(&found, kern, &probe);
+            }
+            if (e != cudaSuccess) {
+                (void)cudaGetLastError();  // do not leave the error behind for an unrelated later call
+                return e;
+            }
+            found = std::min(PAIR ? std::min(found, sms / 2) : sms, max_workers(s));
+            if (found < 1)
+                return cudaErrorNotSupported;
+            known = found;
+        }
+        workers = known;
+    }
+    config.gridDim = dim3(PAIR ? 2 * workers : workers);
+    e              = cudaLaunchKernelEx(&config, kern, p);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
@@ -156,7 +187,7 @@ cudaError_t linear(cudaStream_t stream, LinearShape s, const void* A, const floa
         return cudaErrorInvalidValue;
     choose_tiles(s);
     // even a table of borders that is corrupt must not overflow the tile numbers
-    const long tiles_m = (s.m - 1) / kLinearRows + 1, tiles_n = (s.n - 1) / s.nt + 1;
+    const long tiles_m = (s.m - 1) / (s.pair ? kPairTile : kLinearRows) + 1, tiles_n = (s.n - 1) / s.nt + 1;
     if (tiles_m * tiles_n > 0x7fffffffL / s.groups)
         return cudaErrorInvalidValue;
 
@@ -175,7 +206,6 @@ cudaError_t linear(cudaStream_t stream, LinearShape s, const void* A, const floa
     p.m        = s.m;
     p.n        = s.n;
     p.kb       = s.kb;
-    p.steps    = (s.kb - 1) / kStepBlocks + 1;
     p.nt       = s.nt;
     p.b_box    = s.b_box;
     p.bf16     = C_type == SPMM_B200_BF16;
@@ -183,9 +213,12 @@ cudaError_t linear(cudaStream_t stream, LinearShape s, const void* A, const floa
     if (workspace && workspace_bytes >= workspace_needed(s)) {
         p.counters = static_cast<unsigned*>(workspace);
         p.slots    = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
-        p.overhead = 2;
+        p.overhead = s.pair ? 16 : 2;
     }
-    return s.eight ? launch<true>(stream, p, s) : launch<false>(stream, p, s);
+    p.wide_c = aligned16(C) && s.m % 8 == 0;
+    if (s.pair)
+        return s.eight ? launch<true, true>(stream, p, s) : launch<false, true>(stream, p, s);
+    return s.eight ? launch<true, false>(stream, p, s) : launch<false, false>(stream, p, s);
 }
 
 LinearShape shape_of(bool eight, bool ragged, int groups, int m, int n, int k)

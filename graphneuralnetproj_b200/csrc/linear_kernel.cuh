@@ -43,6 +43,7 @@ constexpr int kStepBlocks      = 2;  // k-blocks per ring stage
 constexpr int kGroupBlocks     = 8;  // k-blocks of a group at most
 constexpr int kGroupScales     = 256;  // scales of a group: k-blocks x columns
 constexpr int kEpilogueTeams   = 8;  // epilogue warps
+constexpr int kLinearBand      = 8;
 constexpr int kPieceCounters   = 4096;  // arrival counters at the head of a workspace
 constexpr int kLinearFixedSmem = 1024 /* alignment */ + 512 /* barriers */;
 
@@ -61,6 +62,7 @@ struct LinearParams {
     int          b_box;     // tokens per TMA box
     int          stages;
     int          bf16;      // C (and 16-bit operands) are bf16, not fp16
+    int          wide_c;    // C takes 16-byte stores: aligned, M a multiple of 8
     int          overhead;  // see make_linear_partition
 };
 
@@ -68,6 +70,124 @@ struct LinearParams {
 struct LinearTile {
     int group, m0, row0, rows;  // first row of A, first token, tokens
 };
+
+// One element of C, rounded once.
+__device__ __forceinline__ void linear_store(const LinearParams& p, size_t at, float v)
+{
+    if (p.bf16)
+        static_cast<__nv_bfloat16*>(p.C)[at] = __float2bfloat16_rn(v);
+    else
+        static_cast<half*>(p.C)[at] = __float2half_rn(v);
+}
+
+// Two of them.
+__device__ __forceinline__ uint32_t linear_pair_of(float lo, float hi, int bf16)
+{
+    uint32_t out;
+    if (bf16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        out                    = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    else {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        out             = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return out;
+}
+
+// The groups, as every role of a block needs them (in shared memory).
+struct LinearTable {
+    int* end;   // tiles of the groups up to and including this one
+    int* row;   // first token
+    int* rows;  // tokens
+};
+
+// Fills the table; all threads of the block, with two block barriers.  Borders are clamped to the tokens there are, so
+// that a corrupt table cannot lead outside.  Tiles are `tile_tokens` tokens x one of `tiles_m` blocks of rows of A.
+__device__ __forceinline__ void
+linear_build_table(const LinearParams& p, const LinearTable& table, int* warp_sums, int tile_tokens, int tiles_m)
+{
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int per  = (p.groups + kLinearThreads - 1) / kLinearThreads;
+    const int e0   = min(static_cast<int>(threadIdx.x) * per, p.groups), e1 = min(e0 + per, p.groups);
+    int       sum  = 0;
+    for (int e = e0; e < e1; e++) {
+        int from = 0, rows = p.n;
+        if (p.offsets) {
+            from = min(max(__ldg(p.offsets + e), 0), p.n);
+            rows = max(min(max(__ldg(p.offsets + e + 1), 0), p.n) - from, 0);
+        }
+        table.row[e]  = from;
+        table.rows[e] = rows;
+        sum += (rows + tile_tokens - 1) / tile_tokens * tiles_m;
+        table.end[e] = sum;
+    }
+    int before = sum;  // becomes the total of the threads before this one
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, before, d);
+        if (lane >= d)
+            before += up;
+    }
+    if (lane == 31)
+        warp_sums[warp] = before;
+    before -= sum;
+    __syncthreads();
+    for (int w = 0; w < warp; w++)
+        before += warp_sums[w];
+    for (int e = e0; e < e1; e++)
+        table.end[e] += before;
+    __syncthreads();
+}
+
+// Which part of the layer a tile is: `block_rows` rows of A and up to `tile_tokens` tokens.  Tiles that run at the same time
+// should share operands in L2: tokens are taken in bands of kLinearBand tiles, in a band a block of rows of A after the other.
+__device__ __forceinline__ LinearTile
+linear_locate(const LinearParams& p, const LinearTable& table, int tile, int tile_tokens, int block_rows, int tiles_m)
+{
+    int lo = 0, hi = p.groups - 1;  // the first group whose running total is above `tile`
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (table.end[mid] > tile)
+            hi = mid;
+        else
+            lo = mid + 1;
+    }
+    LinearTile t;
+    const int  rows = table.rows[lo], tiles_n = (rows + tile_tokens - 1) / tile_tokens;
+    const int  i    = tile - (lo > 0 ? table.end[lo - 1] : 0);
+    const int  band = i / (kLinearBand * tiles_m), wide = min(kLinearBand, tiles_n - band * kLinearBand);
+    const int  rest = i - band * kLinearBand * tiles_m;
+    t.group = lo;
+    t.m0    = rest / wide * block_rows;
+    t.row0  = (band * kLinearBand + rest % wide) * tile_tokens;
+    t.rows  = min(tile_tokens, rows - t.row0);
+    t.row0 += table.row[lo];
+    return t;
+}
+
+// The value of lane 0, known to the compiler to be the same in all lanes.
+__device__ __forceinline__ int linear_uniform(int v)
+{
+    return __shfl_sync(0xffffffffu, v, 0);
+}
+
+// Segments and tiles for the warps that issue MMAs and TMA loads (see ptx::elect_one).
+__device__ __forceinline__ LinearSegment linear_uniform(LinearSegment s)
+{
+    s.tile = linear_uniform(s.tile);
+    s.kb0  = linear_uniform(s.kb0);
+    s.kb1  = linear_uniform(s.kb1);
+    return s;
+}
+__device__ __forceinline__ LinearTile linear_uniform(LinearTile t)
+{
+    t.group = linear_uniform(t.group);
+    t.m0    = linear_uniform(t.m0);
+    t.row0  = linear_uniform(t.row0);
+    t.rows  = linear_uniform(t.rows);
+    return t;
+}
 
 // Steps whose products fit side by side into 256 TMEM columns, and the columns of each.
 SPMM_B200_HD int linear_group_steps(int nt)
@@ -128,11 +248,10 @@ linear_kernel(const __grid_constant__ LinearParams p)
     volatile uint32_t* tmem_slot  = reinterpret_cast<volatile uint32_t*>(smem + bar_off + kWords);
     volatile int*      abort_word = reinterpret_cast<volatile int*>(smem + bar_off + kWords + 4);
     int* const         warp_sums  = reinterpret_cast<int*>(smem + bar_off + kWords + 8);  // 12 words
-    int* const         tile_end   = reinterpret_cast<int*>(smem + bar_off + 512);         // per group, running total
-    int* const         group_row  = tile_end + p.groups;                                  // first token
-    int* const         group_rows = group_row + p.groups;                                 // tokens
+    int* const         groups_at  = reinterpret_cast<int*>(smem + bar_off + 512);
+    const LinearTable  table{groups_at, groups_at + p.groups, groups_at + 2 * p.groups};
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = linear_uniform(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kLinearMaxStages; s++) {
@@ -153,87 +272,37 @@ linear_kernel(const __grid_constant__ LinearParams p)
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
 
-    // Tiles per group.  Borders are clamped to the tokens there are, so that a corrupt table cannot lead outside.
     const int tiles_m = (p.m - 1) / kLinearRows + 1;
-    {
-        const int per = (p.groups + kLinearThreads - 1) / kLinearThreads;
-        const int e0  = min(static_cast<int>(threadIdx.x) * per, p.groups), e1 = min(e0 + per, p.groups);
-        int       sum = 0;
-        for (int e = e0; e < e1; e++) {
-            int from = 0, rows = p.n;
-            if (p.offsets) {
-                from = min(max(__ldg(p.offsets + e), 0), p.n);
-                rows = max(min(max(__ldg(p.offsets + e + 1), 0), p.n) - from, 0);
-            }
-            group_row[e]  = from;
-            group_rows[e] = rows;
-            sum += (rows + p.nt - 1) / p.nt * tiles_m;
-            tile_end[e] = sum;
-        }
-        int before = sum;  // becomes the total of the threads before this one
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int up = __shfl_up_sync(0xffffffffu, before, d);
-            if (lane >= d)
-                before += up;
-        }
-        if (lane == 31)
-            warp_sums[warp] = before;
-        before -= sum;
-        ptx::tc_fence_before_sync();
-        __syncthreads();
-        for (int w = 0; w < warp; w++)
-            before += warp_sums[w];
-        for (int e = e0; e < e1; e++)
-            tile_end[e] += before;
-        __syncthreads();
-        ptx::tc_fence_after_sync();
-    }
-    const uint32_t        tmem_base = *tmem_slot;
-    const LinearPartition part      = make_linear_partition(tile_end[p.groups - 1], p.steps, static_cast<int>(gridDim.x), p.overhead);
+    ptx::tc_fence_before_sync();
+    linear_build_table(p, table, warp_sums, p.nt, tiles_m);
+    ptx::tc_fence_after_sync();
+    const uint32_t        tmem_base = linear_uniform(static_cast<int>(*tmem_slot));
+    const LinearPartition part      = make_linear_partition(table.end[p.groups - 1], p.steps, static_cast<int>(gridDim.x), p.overhead);
     const int             worker    = static_cast<int>(blockIdx.x);
 
-    auto locate = [&](int tile) {
-        int lo = 0, hi = p.groups - 1;  // the first group whose running total is above `tile`
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (tile_end[mid] > tile)
-                hi = mid;
-            else
-                lo = mid + 1;
-        }
-        LinearTile t;
-        const int  rows = group_rows[lo], tiles_n = (rows + p.nt - 1) / p.nt;
-        const int  i    = tile - (lo > 0 ? tile_end[lo - 1] : 0);
-        t.group = lo;
-        t.m0    = i / tiles_n * kLinearRows;
-        t.row0  = i % tiles_n * p.nt;
-        t.rows  = min(p.nt, rows - t.row0);
-        t.row0 += group_row[lo];
-        return t;
-    };
+    auto locate  = [&](int tile) { return linear_locate(p, table, tile, p.nt, kLinearRows, tiles_m); };
     auto columns = [&](const LinearTile& t) { return (t.rows + 15) & ~15; };
 
     int issued = 0;  // ring stages filled (warp 0)
     if (warp == 0) {
         // ------------------------------------------------------------ TMA
-        if (lane == 0) {
-            bool     ok = true;
-            int      s  = 0;
-            uint32_t phase = 1;  // of the stages' "empty" barriers: the first round finds them so
-            for (int i = 0; ok; i++) {
-                const LinearSegment seg = linear_segment(part, worker, i);
-                if (seg.tile < 0)
-                    break;
-                const LinearTile t     = locate(seg.tile);
-                const int        boxes = (columns(t) + p.b_box - 1) / p.b_box;
-                const uint32_t   bytes = kStepBlocks * (kLinearBoxBytes + boxes * p.b_box * 128u);
+        bool     ok = true;
+        int      s  = 0;
+        uint32_t phase = 1;  // of the stages' "empty" barriers: the first round finds them so
+        for (int i = 0; ok; i++) {
+            const LinearSegment seg = linear_uniform(linear_segment(part, worker, i));
+            if (seg.tile < 0)
+                break;
+            const LinearTile t     = linear_uniform(locate(seg.tile));
+            const int        boxes = (columns(t) + p.b_box - 1) / p.b_box;
+            const uint32_t   bytes = kStepBlocks * (kLinearBoxBytes + boxes * p.b_box * 128u);
 #pragma unroll 1
-                for (int k = seg.kb0; k < seg.kb1; k++) {
-                    ok = linear_wait(empty(s), phase, abort_word);
-                    if (!ok)
-                        break;
-                    const uint32_t dst = smem_base + s * stage_bytes;
+            for (int k = seg.kb0; k < seg.kb1; k++) {
+                ok = linear_wait(empty(s), phase, abort_word);
+                if (!ok)
+                    break;
+                const uint32_t dst = smem_base + s * stage_bytes;
+                if (ptx::elect_one()) {
                     ptx::mbar_arrive_expect_tx(full(s), bytes);
 #pragma unroll
                     for (int h = 0; h < kStepBlocks; h++) {
@@ -243,47 +312,47 @@ linear_kernel(const __grid_constant__ LinearParams p)
                             ptx::tma_load_3d(dst + kStepBlocks * kLinearBoxBytes + h * part_bytes + b * p.b_box * 128, &p.b_map, x,
                                              t.row0 + b * p.b_box, 0, full(s));
                     }
-                    issued++;
-                    if (++s == p.stages) {
-                        s = 0;
-                        phase ^= 1;
-                    }
+                }
+                issued++;
+                if (++s == p.stages) {
+                    s = 0;
+                    phase ^= 1;
                 }
             }
         }
     }
     else if (warp == 1) {
         // ------------------------------------------------------------ MMA
-        if (lane == 0) {
-            bool           ok  = true;
-            int            s   = 0;
-            uint32_t       phase = 0, use = 0;  // use: halves of TMEM handed over
-            const uint64_t a_desc0 = ptx::make_smem_desc(smem_base, 16, 1024, ptx::kSwizzle128B);
-            for (int i = 0; ok; i++) {
-                const LinearSegment seg = linear_segment(part, worker, i);
-                if (seg.tile < 0)
-                    break;
-                const uint32_t idesc =
-                    ptx::make_idesc_f16_f32(kLinearRows, columns(locate(seg.tile)), false, false) | (!EIGHT && p.bf16 ? ptx::kIdescBf16 : 0u);
-                int      left   = 0;  // steps that the current half still takes
-                uint32_t d_tmem = 0;
+        bool           ok    = true;
+        int            s     = 0;
+        uint32_t       phase = 0, use = 0;  // use: halves of TMEM handed over
+        const uint64_t a_desc0 = ptx::make_smem_desc(smem_base, 16, 1024, ptx::kSwizzle128B);
+        for (int i = 0; ok; i++) {
+            const LinearSegment seg = linear_uniform(linear_segment(part, worker, i));
+            if (seg.tile < 0)
+                break;
+            const uint32_t idesc = ptx::make_idesc_f16_f32(kLinearRows, linear_uniform(columns(locate(seg.tile))), false, false)
+                                   | (!EIGHT && p.bf16 ? ptx::kIdescBf16 : 0u);
+            int      left   = 0;  // steps that the current half still takes
+            uint32_t d_tmem = 0;
 #pragma unroll 1
-                for (int k = seg.kb0; k < seg.kb1; k++) {
-                    const bool fresh = left == 0;
-                    if (fresh) {
-                        left = EIGHT ? min(group_steps, seg.kb1 - k) : seg.kb1 - k;
-                        ok   = linear_wait(acc_free(use & 1), ((use >> 1) & 1) ^ 1, abort_word);
-                        if (!ok)
-                            break;
-                    }
-                    ok = linear_wait(full(s), phase, abort_word);
+            for (int k = seg.kb0; k < seg.kb1; k++) {
+                const bool fresh = left == 0;
+                if (fresh) {
+                    left   = EIGHT ? min(group_steps, seg.kb1 - k) : seg.kb1 - k;
+                    d_tmem = tmem_base + (use & 1) * kGroupScales;
+                    ok     = linear_wait(acc_free(use & 1), ((use >> 1) & 1) ^ 1, abort_word);
                     if (!ok)
                         break;
-                    ptx::tc_fence_after_sync();
-                    if (fresh)
-                        d_tmem = tmem_base + (use & 1) * kGroupScales;
-                    const uint64_t a_desc = a_desc0 + static_cast<uint64_t>((s * stage_bytes) >> 4);
-                    const uint64_t b_desc = a_desc + (kStepBlocks * kLinearBoxBytes >> 4);
+                }
+                ok = linear_wait(full(s), phase, abort_word);
+                if (!ok)
+                    break;
+                ptx::tc_fence_after_sync();
+                const uint64_t a_desc = a_desc0 + static_cast<uint64_t>((s * stage_bytes) >> 4);
+                const uint64_t b_desc = a_desc + (kStepBlocks * kLinearBoxBytes >> 4);
+                left--;
+                if (ptx::elect_one()) {
 #pragma unroll
                     for (int h = 0; h < kStepBlocks; h++)
 #pragma unroll
@@ -295,16 +364,16 @@ linear_kernel(const __grid_constant__ LinearParams p)
                                 ptx::umma_f16_ss(d_tmem, a, b, idesc, !fresh || h > 0 || j > 0);
                         }
                     ptx::umma_commit(empty(s));
-                    if (EIGHT)
-                        d_tmem += kStepBlocks * acc_width;
-                    if (--left == 0) {
+                    if (left == 0)
                         ptx::umma_commit(acc_full(use & 1));
-                        use++;
-                    }
-                    if (++s == p.stages) {
-                        s = 0;
-                        phase ^= 1;
-                    }
+                }
+                if (EIGHT)
+                    d_tmem += kStepBlocks * acc_width;
+                if (left == 0)
+                    use++;
+                if (++s == p.stages) {
+                    s = 0;
+                    phase ^= 1;
                 }
             }
         }
@@ -456,13 +525,8 @@ linear_kernel(const __grid_constant__ LinearParams p)
 #pragma unroll
                 for (int j = 0; j < CH; j++) {
                     const int token = col_of(c) + j;
-                    if (token < t.rows) {
-                        const size_t at = static_cast<size_t>(t.row0 + token) * p.m + m;
-                        if (p.bf16)
-                            static_cast<__nv_bfloat16*>(p.C)[at] = __float2bfloat16_rn(v[j]);
-                        else
-                            static_cast<half*>(p.C)[at] = __float2half_rn(v[j]);
-                    }
+                    if (token < t.rows)
+                        linear_store(p, static_cast<size_t>(t.row0 + token) * p.m + m, v[j]);
                 }
             };
             if (seg.slot < 0) {
@@ -534,7 +598,7 @@ linear_kernel(const __grid_constant__ LinearParams p)
 
     // ---------------------------------------------------------------- exit
     __syncwarp();
-    if (warp == 0 && lane == 0 && *abort_word != 0)  // copies still under way land before the block's memory goes
+    if (warp == 0 && *abort_word != 0)  // copies still under way land before the block's memory goes
         for (int i = max(0, issued - p.stages); i < issued; i++)
             ptx::mbar_wait_quiet(full(i % p.stages), (i / p.stages) & 1, 10000000ull);
     ptx::tc_fence_before_sync();

@@ -1,0 +1,391 @@
+// The linear layers of linear_kernel.cuh at token counts where the tensor core is the bound: tiles of 256 x 256 on pairs of
+// SMs (tcgen05.mma.cta_group::2, a cluster of two blocks).
+//
+// Per k-block (128 bytes of K) the pair MMA takes 512 cycles, in which each block has to bring in 32 KB: 128 rows of the
+// operand on the accumulator's lanes and half of the 256 of the operand on its columns.  One block alone would have to
+// bring in 48 KB in the same time, more than L2 hands to an SM.
+//
+// 16-bit operands: weights on the lanes, tokens as columns, as in the single-block kernel -- the columns of the last tile
+// of a group are cut to its tokens (in steps of 32).
+// Codes: tokens on the lanes, weights as columns.  Every k-block is a product of its own that the epilogue warps add to
+// fp32 registers (128 of them per thread: two warpgroups share the 256 columns) while the tensor core fills the other
+// half of TMEM.  This way round a thread's factor is one number per k-block, (its token's scale) * (the scale of its 128
+// columns), and the addition two columns per instruction; with tokens as columns each column needs its own factor out of
+// shared memory, which costs as much of shared memory's time as the operands do.
+//
+// Roles per block as in the single-block kernel without the scale warp; the even block's (the leader's) warp 1 issues the
+// pair's MMAs.  The "full" and "acc_free" barriers live in the leader; commits arrive in both blocks.  Every wait is
+// bounded, and both blocks meet at a cluster barrier before they exit.
+#pragma once
+
+#include "linear_kernel.cuh"
+
+namespace spmm_b200 {
+
+constexpr int kPairTile       = 256;  // rows of A and tokens of a tile
+constexpr int kPairStageBytes = 2 * kLinearBoxBytes;
+constexpr int kPairStages     = 7;  // at most
+
+template<bool EIGHT>
+__global__ void __launch_bounds__(kLinearThreads, 1)
+linear_pair_kernel(const __grid_constant__ LinearParams p)
+{
+    constexpr int CH  = EIGHT ? 32 : 16;           // columns per chunk
+    constexpr int NCH = kPairTile / (2 * CH);      // chunks per epilogue warp
+
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (ptx::smem_addr(smem_raw) + 1023u) & ~1023u;
+    uint8_t*       smem      = smem_raw + (smem_base - ptx::smem_addr(smem_raw));
+    const uint32_t bar_off   = p.stages * kPairStageBytes;
+    const uint32_t bar_base  = smem_base + bar_off;
+    auto full     = [&](int s) { return bar_base + 8u * s; };                        // the leader's
+    auto empty    = [&](int s) { return bar_base + 8u * (kPairStages + s); };        // each block's own
+    auto acc_full = [&](int b) { return bar_base + 8u * (2 * kPairStages + b); };    // each block's own
+    auto acc_free = [&](int b) { return bar_base + 8u * (2 * kPairStages + 2 + b); };  // the leader's
+    constexpr uint32_t kWords = 8u * (2 * kPairStages + 4);
+    volatile uint32_t* tmem_slot  = reinterpret_cast<volatile uint32_t*>(smem + bar_off + kWords);
+    volatile int*      abort_word = reinterpret_cast<volatile int*>(smem + bar_off + kWords + 4);
+    int* const         warp_sums  = reinterpret_cast<int*>(smem + bar_off + kWords + 8);
+    int* const         groups_at  = reinterpret_cast<int*>(smem + bar_off + 512);
+    const LinearTable  table{groups_at, groups_at + p.groups, groups_at + 2 * p.groups};
+    static_assert(kWords + 64 <= 512, "barrier block");
+
+    const int      warp = linear_uniform(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31;
+    const uint32_t rank = ptx::cluster_cta_rank();  // 0: leader
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kPairStages; s++) {
+            ptx::mbar_init(full(s), 1);
+            ptx::mbar_init(empty(s), 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            ptx::mbar_init(acc_full(b), 1);
+            ptx::mbar_init(acc_free(b), 2 * kEpilogueTeams);
+        }
+        *abort_word = 0;
+        ptx::mbar_init_fence();
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc_pair(bar_base + kWords, 512);
+        ptx::tmem_relinquish_pair();
+    }
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();
+    const int tiles_m = (p.m - 1) / kPairTile + 1;
+    ptx::tc_fence_before_sync();
+    linear_build_table(p, table, warp_sums, kPairTile, tiles_m);
+    ptx::cluster_sync_all();  // both blocks' barriers exist before anyone arrives on the partner's
+    ptx::tc_fence_after_sync();
+    const uint32_t        tmem_base = linear_uniform(static_cast<int>(*tmem_slot));
+    const int             worker    = static_cast<int>(blockIdx.x >> 1);
+    const LinearPartition part = make_linear_partition(table.end[p.groups - 1], p.steps, static_cast<int>(gridDim.x >> 1), p.overhead);
+
+    auto locate = [&](int tile) { return linear_locate(p, table, tile, kPairTile, kPairTile, tiles_m); };
+    // columns of the accumulator that are used
+    auto columns = [&](const LinearTile& t) { return EIGHT ? kPairTile : (t.rows + 31) & ~31; };
+
+    int issued = 0;
+    if (warp < 4) {
+        if (EIGHT)
+            ptx::registers_down<72>();
+        if (warp == 0) {
+            // ------------------------------------------------------------ TMA: this block's part of both operands
+            bool           ok    = true;
+            int            s     = 0;
+            uint32_t       phase = 1;
+            const uint32_t leader_full0 = ptx::map_to_cta(full(0), 0);
+            for (int i = 0; ok; i++) {
+                const LinearSegment seg = linear_uniform(linear_segment(part, worker, i));
+                if (seg.tile < 0)
+                    break;
+                const LinearTile t     = linear_uniform(locate(seg.tile));
+                const int        half  = columns(t) / 2;
+                const int        boxes = EIGHT ? 1 : (half + p.b_box - 1) / p.b_box;
+                const int        m     = t.m0 + static_cast<int>(rank) * kLinearRows;
+                const int        token = t.row0 + static_cast<int>(rank) * (EIGHT ? kLinearRows : half);
+                const uint32_t   bytes = 2 * (kLinearBoxBytes + (EIGHT ? kLinearBoxBytes : boxes * p.b_box * 128));
+#pragma unroll 1
+                for (int k = seg.kb0; k < seg.kb1; k++) {
+                    ok = linear_wait(empty(s), phase, abort_word);
+                    if (!ok)
+                        break;
+                    const uint32_t lanes = smem_base + s * kPairStageBytes, cols = lanes + kLinearBoxBytes;
+                    const uint32_t bar   = leader_full0 + 8u * s;
+                    if (ptx::elect_one()) {
+                        if (rank == 0)
+                            ptx::mbar_arrive_expect_tx(full(s), bytes);  // both blocks' bytes
+                        ptx::tma_load_3d_pair(EIGHT ? cols : lanes, &p.a_map, k * 128, m, t.group, bar);
+                        if (EIGHT)
+                            ptx::tma_load_3d_pair(lanes, &p.b_map, k * 128, token, 0, bar);
+                        else
+                            for (int b = 0; b < boxes; b++)
+                                ptx::tma_load_3d_pair(cols + b * p.b_box * 128, &p.b_map, k * 128, token + b * p.b_box, 0, bar);
+                    }
+                    issued++;
+                    if (++s == p.stages) {
+                        s = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+        }
+        else if (warp == 1 && rank == 0) {
+            // ------------------------------------------------------------ leader: MMA for the pair
+            bool           ok    = true;
+            int            s     = 0;
+            uint32_t       phase = 0, use = 0;
+            const uint64_t desc0 = ptx::make_smem_desc(smem_base, 16, 1024, ptx::kSwizzle128B);
+            for (int i = 0; ok; i++) {
+                const LinearSegment seg = linear_uniform(linear_segment(part, worker, i));
+                if (seg.tile < 0)
+                    break;
+                const uint32_t idesc = ptx::make_idesc_f16_f32(kPairTile, linear_uniform(columns(locate(seg.tile))), false, false)
+                                       | (!EIGHT && p.bf16 ? ptx::kIdescBf16 : 0u);
+#pragma unroll 1
+                for (int k = seg.kb0; k < seg.kb1; k++) {
+                    const bool fresh = EIGHT || k == seg.kb0, last = EIGHT || k == seg.kb1 - 1;
+                    if (fresh)
+                        ok = linear_wait(acc_free(use & 1), ((use >> 1) & 1) ^ 1, abort_word);
+                    ok = ok && linear_wait(full(s), phase, abort_word);
+                    if (!ok)
+                        break;
+                    ptx::tc_fence_after_sync();
+                    const uint32_t d_tmem = tmem_base + (use & 1) * kPairTile;
+                    const uint64_t a_desc = desc0 + static_cast<uint64_t>(s * (kPairStageBytes >> 4));
+                    const uint64_t b_desc = a_desc + (kLinearBoxBytes >> 4);
+                    if (ptx::elect_one()) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            if (EIGHT)
+                                ptx::umma_f8_ss_pair(d_tmem, a_desc + j * 2, b_desc + j * 2, idesc, j > 0);
+                            else
+                                ptx::umma_f16_ss_pair(d_tmem, a_desc + j * 2, b_desc + j * 2, idesc, !fresh || j > 0);
+                        }
+                        ptx::umma_commit_both(empty(s));
+                        if (last)
+                            ptx::umma_commit_both(acc_full(use & 1));
+                    }
+                    if (last)
+                        use++;
+                    if (++s == p.stages) {
+                        s = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+        }
+    }
+    else {
+        if (EIGHT)
+            ptx::registers_up<216>();
+        // ------------------------------------------------------------ epilogue: this block's 128 lanes
+        const int      team    = (warp - 4) >> 2;
+        const int      row     = (warp & 3) * 32 + lane;
+        const uint32_t tmem_at = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        const uint32_t leader_acc_free0 = ptx::map_to_cta(acc_free(0), 0);
+        auto           col_of  = [&](int c) { return EIGHT ? team * 128 + c * CH : (2 * c + team) * CH; };
+        uint32_t       use     = 0;
+        bool           ok      = true;
+        for (int i = 0; ok; i++) {
+            const LinearSegment seg = linear_segment(part, worker, i);
+            if (seg.tile < 0)
+                break;
+            const LinearTile t = locate(seg.tile);
+            const int        n = columns(t);
+            const int        token = static_cast<int>(rank) * kLinearRows + row;  // of this lane (codes)
+            uint64_t         acc[EIGHT ? kPairTile / 4 : 1];  // two fp32 sums each
+            if constexpr (EIGHT) {
+#pragma unroll
+                for (int c = 0; c < kPairTile / 4; c++)
+                    acc[c] = 0;
+                // Factors: the token's scales are loaded four k-blocks at a time, four to eight ahead of their use; the
+                // weights' come 32 k-blocks at a time, one per lane.
+                const int    blocks_m = (p.m - 1) / kLinearRows + 1;
+                const int    m_block  = min(t.m0 / kLinearRows + team, blocks_m - 1);
+                const float* sa       = p.a_scales + (static_cast<size_t>(t.group) * blocks_m + m_block) * p.kb;
+                const float* sb       = p.b_scales + t.row0 + min(token, t.rows - 1);
+                float        ahead[4], now[4], a_ahead = __ldg(sa + min(seg.kb0 + lane, p.kb - 1)), a_now = 0.0f;
+                auto         fetch = [&](int k) {
+#pragma unroll
+                    for (int u = 0; u < 4; u++)
+                        ahead[u] = __ldg(sb + static_cast<size_t>(min(k + u, p.kb - 1)) * p.n);
+                };
+                fetch(seg.kb0);
+#pragma unroll 1
+                for (int k = seg.kb0; k < seg.kb1; k++, use++) {
+                    const int at = k - seg.kb0;
+                    if ((at & 3) == 0) {
+#pragma unroll
+                        for (int u = 0; u < 4; u++)
+                            now[u] = ahead[u];
+                        fetch(k + 4);
+                    }
+                    if ((at & 31) == 0) {
+                        a_now   = a_ahead;
+                        a_ahead = __ldg(sa + min(k + 32 + lane, p.kb - 1));
+                    }
+                    const float    b_scale = (at & 2) ? ((at & 1) ? now[3] : now[2]) : ((at & 1) ? now[1] : now[0]);
+                    const float    factor  = b_scale * __shfl_sync(0xffffffffu, a_now, at & 31);
+                    const uint64_t factor2 = ptx::pack_x2(__float_as_uint(factor), __float_as_uint(factor));
+                    ok = linear_wait(acc_full(use & 1), (use >> 1) & 1, abort_word);
+                    if (!ok)
+                        break;
+                    ptx::tc_fence_after_sync();
+                    const uint32_t from = tmem_at + (use & 1) * kPairTile;
+                    uint32_t       product[2][CH];
+                    ptx::tmem_ld_x32(from + col_of(0), product[0]);
+#pragma unroll
+                    for (int c = 0; c < NCH; c++) {
+                        ptx::tmem_ld_wait();
+                        if (c + 1 < NCH)
+                            ptx::tmem_ld_x32(from + col_of(c + 1), product[(c + 1) & 1]);
+                        else {
+                            ptx::tc_fence_before_sync();
+                            __syncwarp();
+                            if (lane == 0)
+                                ptx::mbar_arrive_remote(leader_acc_free0 + 8u * (use & 1));
+                        }
+#pragma unroll
+                        for (int j = 0; j < CH / 2; j++)
+                            acc[c * (CH / 2) + j] = ptx::fma_x2(ptx::pack_x2(product[c & 1][2 * j], product[c & 1][2 * j + 1]), factor2,
+                                                                acc[c * (CH / 2) + j]);
+                    }
+                }
+            }
+            else {
+                ok = linear_wait(acc_full(use & 1), (use >> 1) & 1, abort_word);
+                ptx::tc_fence_after_sync();
+            }
+            if (!ok)
+                break;
+            auto values = [&](int c, float* v) {
+                if constexpr (EIGHT) {
+#pragma unroll
+                    for (int j = 0; j < CH / 2; j++) {
+                        uint32_t lo, hi;
+                        ptx::unpack_x2(acc[c * (CH / 2) + j], lo, hi);
+                        v[2 * j]     = __uint_as_float(lo);
+                        v[2 * j + 1] = __uint_as_float(hi);
+                    }
+                }
+                else {
+                    uint32_t chunk[CH];
+                    ptx::tmem_ld_x16(tmem_at + (use & 1) * kPairTile + col_of(c), chunk);
+                    ptx::tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < CH; j++)
+                        v[j] = __uint_as_float(chunk[j]);
+                }
+            };
+            auto store = [&](int c, const float* v) {
+                if (EIGHT) {  // one token's columns
+                    const int m = t.m0 + col_of(c);
+                    if (token >= t.rows || m >= p.m)
+                        return;
+                    const size_t at = static_cast<size_t>(t.row0 + token) * p.m + m;
+                    if (p.wide_c && m + CH <= p.m) {
+                        uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.C) + at);
+#pragma unroll
+                        for (int j = 0; j < CH / 8; j++)
+                            to[j] = make_uint4(linear_pair_of(v[8 * j], v[8 * j + 1], p.bf16), linear_pair_of(v[8 * j + 2], v[8 * j + 3], p.bf16),
+                                               linear_pair_of(v[8 * j + 4], v[8 * j + 5], p.bf16), linear_pair_of(v[8 * j + 6], v[8 * j + 7], p.bf16));
+                        return;
+                    }
+#pragma unroll
+                    for (int j = 0; j < CH; j++)
+                        if (m + j < p.m)
+                            linear_store(p, at + j, v[j]);
+                    return;
+                }
+                const int m = t.m0 + static_cast<int>(rank) * kLinearRows + row;
+                if (m >= p.m)
+                    return;
+#pragma unroll
+                for (int j = 0; j < CH; j++)
+                    if (col_of(c) + j < t.rows)
+                        linear_store(p, static_cast<size_t>(t.row0 + col_of(c) + j) * p.m + m, v[j]);
+            };
+            if (seg.slot < 0) {
+#pragma unroll
+                for (int c = 0; c < NCH; c++)
+                    if (col_of(c) < n) {
+                        float v[CH];
+                        values(c, v);
+                        store(c, v);
+                    }
+            }
+            else {
+                constexpr size_t kSlot4 = static_cast<size_t>(kLinearRows) * kPairTile / 4;
+                float4* const    slots  = reinterpret_cast<float4*>(p.slots) + rank * kSlot4 + row;
+                float4* const    mine   = slots + 2 * seg.slot * kSlot4;
+#pragma unroll
+                for (int c = 0; c < NCH; c++)
+                    if (col_of(c) < n) {
+                        float v[CH];
+                        values(c, v);
+#pragma unroll
+                        for (int j = 0; j < CH / 4; j++)
+                            __stcg(mine + (col_of(c) / 4 + j) * kLinearRows, make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+                    }
+                __threadfence();
+                __syncwarp();
+                unsigned  arrived = 0;
+                unsigned* counter = p.counters + (2 * seg.first + rank) * kEpilogueTeams + (warp - 4);
+                if (lane == 0)
+                    arrived = atomicAdd(counter, 1u);
+                arrived = __shfl_sync(0xffffffffu, arrived, 0);
+                if (arrived == static_cast<unsigned>(seg.last - seg.first)) {
+                    if (lane == 0)
+                        *counter = 0;
+                    __threadfence();
+#pragma unroll 1
+                    for (int c = 0; c < NCH; c++)
+                        if (col_of(c) < n) {
+                            float v[CH];
+#pragma unroll
+                            for (int j = 0; j < CH; j++)
+                                v[j] = 0.0f;
+#pragma unroll 1
+                            for (int w = seg.first; w <= seg.last; w++) {
+                                const float4* from = slots + 2 * linear_slot_of(part, seg, w) * kSlot4 + (col_of(c) / 4) * kLinearRows;
+#pragma unroll
+                                for (int j = 0; j < CH / 4; j++) {
+                                    const float4 f = __ldcg(from + j * kLinearRows);
+                                    v[4 * j] += f.x;
+                                    v[4 * j + 1] += f.y;
+                                    v[4 * j + 2] += f.z;
+                                    v[4 * j + 3] += f.w;
+                                }
+                            }
+                            store(c, v);
+                        }
+                }
+            }
+            if (!EIGHT) {
+                ptx::tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0)
+                    ptx::mbar_arrive_remote(leader_acc_free0 + 8u * (use & 1));
+                use++;
+            }
+        }
+    }
+
+    // ---------------------------------------------------------------- exit
+    __syncwarp();
+    if (warp == 0 && rank == 0 && *abort_word != 0)  // both blocks' copies still under way are counted here
+        for (int i = max(0, issued - p.stages); i < issued; i++)
+            ptx::mbar_wait_quiet(full(i % p.stages), (i / p.stages) & 1, 10000000ull);
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    if (threadIdx.x == 0 && *abort_word != 0)
+        atomicExch(&g_linear_status, 1);
+    // Neither block leaves while its partner may still arrive on its barriers or the leader's MMAs read its memory.
+    ptx::cluster_sync_all();
+    if (warp == 1) {
+        ptx::tc_fence_after_sync();
+        ptx::tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
+}  // namespace spmm_b200

@@ -207,6 +207,20 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst_smem, const void* 
                  : "memory");
 }
 
+__device__ __forceinline__ void
+tma_load_3d_pair(uint32_t dst_smem, const void* tensor_map, int x, int y, int z, uint32_t bar_cluster)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            dst_smem),
+        "l"(tensor_map),
+        "r"(x),
+        "r"(y),
+        "r"(z),
+        "r"(bar_cluster)
+        : "memory");
+}
+
 // Asks the memory system to bring `bytes` (a multiple of 16, from a 16-byte aligned address) into L2.
 __device__ __forceinline__ void bulk_prefetch_l2(const void* src, uint32_t bytes)
 {
@@ -421,6 +435,20 @@ umma_f16_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t ide
                  : "memory");
 }
 
+// The same for 8-bit floating-point inputs.
+__device__ __forceinline__ void
+umma_f8_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+                 "l"(a_desc),
+                 "l"(b_desc),
+                 "r"(idesc),
+                 "r"(accumulate)
+                 : "memory");
+}
+
 // Arrives on an mbarrier of either block of the pair (address in the cluster's shared window) once
 // every pair MMA issued so far by this thread has completed.
 __device__ __forceinline__ void umma_commit_pair(uint32_t bar_cluster)
@@ -464,6 +492,74 @@ __device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t* r)
                    "=r"(r[15])
                  : "r"(taddr)
                  : "memory");
+}
+
+// 32 columns.
+__device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t* r)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+                   "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+                   "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr)
+                 : "memory");
+}
+
+// One lane of the warp, the same every time.  Code under it stays uniform for the compiler, unlike code under
+// `lane == 0`, whose operands it has to move to uniform registers one by one for every MMA, commit and TMA load.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
+
+// Arrives on an mbarrier anywhere in the cluster (address from map_to_cta) without ordering other memory accesses of
+// this thread for the other block: for hand-overs of TMEM, which tcgen05 fences order.
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t bar_cluster)
+{
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
+}
+
+// umma_commit_pair for the barriers at this address in both blocks of the pair.
+__device__ __forceinline__ void umma_commit_both(uint32_t bar)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                 "h"(static_cast<uint16_t>(3))
+                 : "memory");
+}
+
+// Moves registers between the warps of a block: every warp of a warpgroup calls it, with the same number.
+template<int N>
+__device__ __forceinline__ void registers_up()
+{
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template<int N>
+__device__ __forceinline__ void registers_down()
+{
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// Two fp32 multiply-adds in one instruction: c + a * b on both halves.
+__device__ __forceinline__ uint64_t fma_x2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t pack_x2(uint32_t lo, uint32_t hi)
+{
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+    return d;
+}
+__device__ __forceinline__ void unpack_x2(uint64_t v, uint32_t& lo, uint32_t& hi)
+{
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
 }
 
 // ---------------------------------------------------------------- descriptors

@@ -130,6 +130,11 @@ GROUPED = [  # m, n, k, group sizes, first row
     (520, 2000, 144, [0] * 30 + [1990] + [0] * 33, 5),  # one group has nearly everything
     (64, 1024, 48, [1] * 1024, 0),                  # as many groups as there may be
     (384, 9, 2064, [0, 0, 0], 4),                   # nothing to do
+    (264, 900, 528, [300, 0, 1, 257, 300], 7),      # many tokens per group: pairs of SMs
+    (1000, 1400, 1040, [1393], 0),
+    (513, 2100, 272, [33, 512, 129, 1400], 3),      # M odd
+    (256, 520, 8192, [257, 263], 0),                # K cut between pairs
+    (128, 700, 16, [160, 540], 0),
 ]
 
 
