@@ -108,7 +108,7 @@ __device__ __forceinline__ void
 linear_build_table(const LinearParams& p, const LinearTable& table, int* warp_sums, int tile_tokens, int tiles_m)
 {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int per  = (p.groups + kLinearThreads - 1) / kLinearThreads;
+    const int per  = (p.groups + static_cast<int>(blockDim.x) - 1) / static_cast<int>(blockDim.x);
     const int e0   = min(static_cast<int>(threadIdx.x) * per, p.groups), e1 = min(e0 + per, p.groups);
     int       sum  = 0;
     for (int e = e0; e < e1; e++) {

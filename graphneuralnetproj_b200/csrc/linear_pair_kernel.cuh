@@ -25,30 +25,42 @@ namespace spmm_b200 {
 constexpr int kPairTile       = 256;  // rows of A and tokens of a tile
 constexpr int kPairStageBytes = 2 * kLinearBoxBytes;
 constexpr int kPairStages     = 7;  // at most
+constexpr int kPairBatch      = 8;  // k-blocks whose factors are handed over together
+
+// Epilogue warps: two warpgroups read 16-bit products out of TMEM once per tile; four share the additions of every k-block.
+template<bool EIGHT>
+constexpr int kPairEpilogueWarps = 8;
+template<bool EIGHT>
+constexpr int kPairThreads = 128 + 32 * kPairEpilogueWarps<EIGHT>;
 
 template<bool EIGHT>
-__global__ void __launch_bounds__(kLinearThreads, 1)
+__global__ void __launch_bounds__(kPairThreads<EIGHT>, 1)
 linear_pair_kernel(const __grid_constant__ LinearParams p)
 {
-    constexpr int CH  = EIGHT ? 32 : 16;           // columns per chunk
-    constexpr int NCH = kPairTile / (2 * CH);      // chunks per epilogue warp
+    constexpr int EPI   = kPairEpilogueWarps<EIGHT>;
+    constexpr int TEAMS = EPI / 4;                   // warps per quarter of the lanes
+    constexpr int CH    = EIGHT ? 32 : 16;           // columns per chunk
+    constexpr int NCH   = kPairTile / (TEAMS * CH);  // chunks per epilogue warp
 
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (ptx::smem_addr(smem_raw) + 1023u) & ~1023u;
     uint8_t*       smem      = smem_raw + (smem_base - ptx::smem_addr(smem_raw));
-    const uint32_t bar_off   = p.stages * kPairStageBytes;
+    const uint32_t scale_off = p.stages * kPairStageBytes;  // factors: [2][kPairBatch][two halves of the columns][128 lanes]
+    const uint32_t bar_off   = scale_off + (EIGHT ? 2 * kPairBatch * 1024u : 0u);
     const uint32_t bar_base  = smem_base + bar_off;
     auto full     = [&](int s) { return bar_base + 8u * s; };                        // the leader's
     auto empty    = [&](int s) { return bar_base + 8u * (kPairStages + s); };        // each block's own
     auto acc_full = [&](int b) { return bar_base + 8u * (2 * kPairStages + b); };    // each block's own
     auto acc_free = [&](int b) { return bar_base + 8u * (2 * kPairStages + 2 + b); };  // the leader's
-    constexpr uint32_t kWords = 8u * (2 * kPairStages + 4);
+    auto scale_full = [&](int b) { return bar_base + 8u * (2 * kPairStages + 4 + b); };  // each block's own
+    auto scale_free = [&](int b) { return bar_base + 8u * (2 * kPairStages + 6 + b); };
+    constexpr uint32_t kWords = 8u * (2 * kPairStages + 8);
     volatile uint32_t* tmem_slot  = reinterpret_cast<volatile uint32_t*>(smem + bar_off + kWords);
     volatile int*      abort_word = reinterpret_cast<volatile int*>(smem + bar_off + kWords + 4);
     int* const         warp_sums  = reinterpret_cast<int*>(smem + bar_off + kWords + 8);
     int* const         groups_at  = reinterpret_cast<int*>(smem + bar_off + 512);
     const LinearTable  table{groups_at, groups_at + p.groups, groups_at + 2 * p.groups};
-    static_assert(kWords + 64 <= 512, "barrier block");
+    static_assert(kWords + 8 + 20 * 4 <= 512, "barrier block");
 
     const int      warp = linear_uniform(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31;
     const uint32_t rank = ptx::cluster_cta_rank();  // 0: leader
@@ -60,7 +72,9 @@ linear_pair_kernel(const __grid_constant__ LinearParams p)
         }
         for (int b = 0; b < 2; b++) {
             ptx::mbar_init(acc_full(b), 1);
-            ptx::mbar_init(acc_free(b), 2 * kEpilogueTeams);
+            ptx::mbar_init(acc_free(b), 2 * EPI);
+            ptx::mbar_init(scale_full(b), 2);
+            ptx::mbar_init(scale_free(b), EPI);
         }
         *abort_word = 0;
         ptx::mbar_init_fence();
@@ -144,9 +158,12 @@ linear_pair_kernel(const __grid_constant__ LinearParams p)
 #pragma unroll 1
                 for (int k = seg.kb0; k < seg.kb1; k++) {
                     const bool fresh = EIGHT || k == seg.kb0, last = EIGHT || k == seg.kb1 - 1;
-                    if (fresh)
+                    const bool free = !fresh || ptx::mbar_test_wait(acc_free(use & 1), ((use >> 1) & 1) ^ 1);
+                    const bool here = ptx::mbar_test_wait(full(s), phase);  // asked at the same time
+                    if (!__all_sync(0xffffffffu, free))
                         ok = linear_wait(acc_free(use & 1), ((use >> 1) & 1) ^ 1, abort_word);
-                    ok = ok && linear_wait(full(s), phase, abort_word);
+                    if (!__all_sync(0xffffffffu, here))
+                        ok = ok && linear_wait(full(s), phase, abort_word);
                     if (!ok)
                         break;
                     ptx::tc_fence_after_sync();
@@ -174,17 +191,73 @@ linear_pair_kernel(const __grid_constant__ LinearParams p)
                 }
             }
         }
+        else if (EIGHT && warp >= 2) {
+            // ------------------------------------------------------------ factors: each of two warps half of a batch's k-blocks
+            // (token's scale) * (scale of its 128 columns), laid out per half of the columns and lane, loaded a batch ahead.
+            constexpr int PER      = kPairBatch / 2;
+            const int     blocks_m = (p.m - 1) / kLinearRows + 1, mine = (warp - 2) * PER;
+            float* const  ring     = reinterpret_cast<float*>(smem + scale_off);
+            int           next_i = 0, next_k = 0;
+            LinearSegment next_seg = linear_segment(part, worker, 0);
+            LinearTile    next_tile{};
+            if (next_seg.tile >= 0) {
+                next_tile = locate(next_seg.tile);
+                next_k    = next_seg.kb0;
+            }
+            float a = 0.0f, b[PER][4];  // lane 4 * h + u of `a`: columns' half h, k-block u
+            auto  fetch = [&]() {
+                if (next_seg.tile < 0)
+                    return false;
+                const int m_block = min(next_tile.m0 / kLinearRows + ((lane >> 2) & 1), blocks_m - 1);
+                a = __ldg(p.a_scales + (static_cast<size_t>(next_tile.group) * blocks_m + m_block) * p.kb
+                          + min(next_k + mine + (lane & 3), p.kb - 1));
+#pragma unroll
+                for (int u = 0; u < PER; u++) {
+                    const float* from = p.b_scales + static_cast<size_t>(min(next_k + mine + u, p.kb - 1)) * p.n + next_tile.row0;
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        b[u][j] = __ldg(from + min(static_cast<int>(rank) * kLinearRows + lane + 32 * j, next_tile.rows - 1));
+                }
+                next_k += kPairBatch;
+                if (next_k >= next_seg.kb1) {
+                    next_seg = linear_segment(part, worker, ++next_i);
+                    if (next_seg.tile >= 0) {
+                        next_tile = locate(next_seg.tile);
+                        next_k    = next_seg.kb0;
+                    }
+                }
+                return true;
+            };
+            bool have = fetch();
+            for (uint32_t use = 0; have; use++) {
+                if (!linear_wait(scale_free(use & 1), ((use >> 1) & 1) ^ 1, abort_word))
+                    break;
+#pragma unroll
+                for (int u = 0; u < PER; u++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const float block_scale = __shfl_sync(0xffffffffu, a, 4 * h + u);
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            ring[((use & 1) * kPairBatch + mine + u) * 256 + h * 128 + lane + 32 * j] = b[u][j] * block_scale;
+                    }
+                __syncwarp();
+                if (lane == 0)
+                    ptx::mbar_arrive(scale_full(use & 1));
+                have = fetch();
+            }
+        }
     }
     else {
         if (EIGHT)
-            ptx::registers_up<216>();
+            ptx::registers_up<216>();  // 128 * 72 + 256 * 216 = 384 * 168, the registers at launch
         // ------------------------------------------------------------ epilogue: this block's 128 lanes
         const int      team    = (warp - 4) >> 2;
         const int      row     = (warp & 3) * 32 + lane;
         const uint32_t tmem_at = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t leader_acc_free0 = ptx::map_to_cta(acc_free(0), 0);
-        auto           col_of  = [&](int c) { return EIGHT ? team * 128 + c * CH : (2 * c + team) * CH; };
-        uint32_t       use     = 0;
+        auto           col_of  = [&](int c) { return EIGHT ? (team * NCH + c) * CH : (TEAMS * c + team) * CH; };
+        uint32_t       use     = 0, batch = 0;
         bool           ok      = true;
         for (int i = 0; ok; i++) {
             const LinearSegment seg = linear_segment(part, worker, i);
@@ -193,64 +266,58 @@ linear_pair_kernel(const __grid_constant__ LinearParams p)
             const LinearTile t = locate(seg.tile);
             const int        n = columns(t);
             const int        token = static_cast<int>(rank) * kLinearRows + row;  // of this lane (codes)
-            uint64_t         acc[EIGHT ? kPairTile / 4 : 1];  // two fp32 sums each
+            float            acc[EIGHT ? NCH * CH : 1];
             if constexpr (EIGHT) {
 #pragma unroll
-                for (int c = 0; c < kPairTile / 4; c++)
-                    acc[c] = 0;
-                // Factors: the token's scales are loaded four k-blocks at a time, four to eight ahead of their use; the
-                // weights' come 32 k-blocks at a time, one per lane.
-                const int    blocks_m = (p.m - 1) / kLinearRows + 1;
-                const int    m_block  = min(t.m0 / kLinearRows + team, blocks_m - 1);
-                const float* sa       = p.a_scales + (static_cast<size_t>(t.group) * blocks_m + m_block) * p.kb;
-                const float* sb       = p.b_scales + t.row0 + min(token, t.rows - 1);
-                float        ahead[4], now[4], a_ahead = __ldg(sa + min(seg.kb0 + lane, p.kb - 1)), a_now = 0.0f;
-                auto         fetch = [&](int k) {
-#pragma unroll
-                    for (int u = 0; u < 4; u++)
-                        ahead[u] = __ldg(sb + static_cast<size_t>(min(k + u, p.kb - 1)) * p.n);
+                for (int c = 0; c < NCH * CH; c++)
+                    acc[c] = 0.0f;
+                const float* const factors = reinterpret_cast<const float*>(smem + scale_off) + team * 128 + row;
+                auto               release = [&]() {  // a batch of factors
+                    __syncwarp();
+                    if (lane == 0)
+                        ptx::mbar_arrive(scale_free(batch & 1));
+                    batch++;
                 };
-                fetch(seg.kb0);
+                auto factor_of = [&](int at) {  // of the segment's k-block `at`; asked for in order
+                    if (at % kPairBatch == 0) {
+                        if (at > 0)
+                            release();
+                        ok = linear_wait(scale_full(batch & 1), (batch >> 1) & 1, abort_word);
+                    }
+                    return factors[((batch & 1) * kPairBatch + at % kPairBatch) * 256];
+                };
+                float factor = factor_of(0);
+                bool  here   = false;  // the product is known to be there
 #pragma unroll 1
-                for (int k = seg.kb0; k < seg.kb1; k++, use++) {
-                    const int at = k - seg.kb0;
-                    if ((at & 3) == 0) {
-#pragma unroll
-                        for (int u = 0; u < 4; u++)
-                            now[u] = ahead[u];
-                        fetch(k + 4);
+                for (int k = seg.kb0; k < seg.kb1 && ok; k++, use++) {
+                    if (!__all_sync(0xffffffffu, here)) {
+                        ok = linear_wait(acc_full(use & 1), (use >> 1) & 1, abort_word);
+                        if (!ok)
+                            break;
                     }
-                    if ((at & 31) == 0) {
-                        a_now   = a_ahead;
-                        a_ahead = __ldg(sa + min(k + 32 + lane, p.kb - 1));
-                    }
-                    const float    b_scale = (at & 2) ? ((at & 1) ? now[3] : now[2]) : ((at & 1) ? now[1] : now[0]);
-                    const float    factor  = b_scale * __shfl_sync(0xffffffffu, a_now, at & 31);
-                    const uint64_t factor2 = ptx::pack_x2(__float_as_uint(factor), __float_as_uint(factor));
-                    ok = linear_wait(acc_full(use & 1), (use >> 1) & 1, abort_word);
-                    if (!ok)
-                        break;
                     ptx::tc_fence_after_sync();
                     const uint32_t from = tmem_at + (use & 1) * kPairTile;
-                    uint32_t       product[2][CH];
-                    ptx::tmem_ld_x32(from + col_of(0), product[0]);
+                    const float    f    = factor;
 #pragma unroll
                     for (int c = 0; c < NCH; c++) {
-                        ptx::tmem_ld_wait();
-                        if (c + 1 < NCH)
-                            ptx::tmem_ld_x32(from + col_of(c + 1), product[(c + 1) & 1]);
-                        else {
+                        uint32_t product[CH];
+                        ptx::tmem_ld_x32_now(from + col_of(c), product);
+                        if (c == NCH - 1) {
                             ptx::tc_fence_before_sync();
                             __syncwarp();
                             if (lane == 0)
                                 ptx::mbar_arrive_remote(leader_acc_free0 + 8u * (use & 1));
+                            // what the next k-block needs is asked for before these additions
+                            here = ptx::mbar_test_wait(acc_full((use + 1) & 1), ((use + 1) >> 1) & 1);
+                            if (k + 1 < seg.kb1)
+                                factor = factor_of(k + 1 - seg.kb0);
                         }
 #pragma unroll
-                        for (int j = 0; j < CH / 2; j++)
-                            acc[c * (CH / 2) + j] = ptx::fma_x2(ptx::pack_x2(product[c & 1][2 * j], product[c & 1][2 * j + 1]), factor2,
-                                                                acc[c * (CH / 2) + j]);
+                        for (int j = 0; j < CH; j++)
+                            acc[c * CH + j] += __uint_as_float(product[j]) * f;
                     }
                 }
+                release();
             }
             else {
                 ok = linear_wait(acc_full(use & 1), (use >> 1) & 1, abort_word);
@@ -261,12 +328,8 @@ linear_pair_kernel(const __grid_constant__ LinearParams p)
             auto values = [&](int c, float* v) {
                 if constexpr (EIGHT) {
 #pragma unroll
-                    for (int j = 0; j < CH / 2; j++) {
-                        uint32_t lo, hi;
-                        ptx::unpack_x2(acc[c * (CH / 2) + j], lo, hi);
-                        v[2 * j]     = __uint_as_float(lo);
-                        v[2 * j + 1] = __uint_as_float(hi);
-                    }
+                    for (int j = 0; j < CH; j++)
+                        v[j] = acc[c * CH + j];
                 }
                 else {
                     uint32_t chunk[CH];
@@ -330,7 +393,7 @@ linear_pair_kernel(const __grid_constant__ LinearParams p)
                 __threadfence();
                 __syncwarp();
                 unsigned  arrived = 0;
-                unsigned* counter = p.counters + (2 * seg.first + rank) * kEpilogueTeams + (warp - 4);
+                unsigned* counter = p.counters + (2 * seg.first + rank) * EPI + (warp - 4);
                 if (lane == 0)
                     arrived = atomicAdd(counter, 1u);
                 arrived = __shfl_sync(0xffffffffu, arrived, 0);
