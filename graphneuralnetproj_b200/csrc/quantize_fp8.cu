@@ -10,10 +10,14 @@
 //
 // Rounding to the nearest value of the *exact* quotient: x * (1 / s) is off by at most two units in the last place of
 // fp32, so the rounding of that product can differ from the rounding of the quotient only where the product lies within
-// a few units of the midpoint between two e4m3 values.  Those elements (about one in 10^5, plus those below the
-// smallest normal e4m3 value) take the slow path: the correctly rounded quotient, and where the remainder is not zero a
-// step of one unit towards the exact quotient if that makes the last bit odd -- a midpoint is a number of five bits and
-// never odd, so the second rounding then sees the right side.
+// a few units of the midpoint between two e4m3 values.  Those elements (about one in 10^5) take the slow path: the
+// correctly rounded quotient, and where the remainder is not zero a step of one unit towards the exact quotient if that
+// makes the last bit odd -- a midpoint is a number of five bits and never odd, so the second rounding then sees the right
+// side.
+//
+// Bound by memory (2 bytes in, 1 out per element) once an element costs about ten instructions.  Dividing every element,
+// or sending the ones below the smallest normal e4m3 value down the slow path (a few per cent of them where some features
+// are much larger than others, so nearly every warp), made it twice as slow.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -38,21 +42,36 @@ __device__ __forceinline__ float element(uint32_t bits16)
     return __half2float(__ushort_as_half(static_cast<unsigned short>(bits16)));
 }
 
-// Largest magnitude among the finite elements, as the 16-bit pattern of its absolute value (patterns of the same sign
-// order like the numbers), in both halves of the result.
+// The pattern of the smallest magnitude that is not finite, in both halves.
 template<bool BF16>
-__device__ __forceinline__ uint32_t amax_bits(uint32_t m, uint32_t v)
+constexpr uint32_t kInfPair = BF16 ? 0x7f807f80u : 0x7c007c00u;
+
+// Largest magnitude of the elements seen, as the 16-bit pattern of its absolute value (patterns of the same sign order like
+// the numbers; infinities and NaN come last), per half.
+__device__ __forceinline__ uint32_t amax_bits(uint32_t m, uint4 v)
 {
-    constexpr uint32_t kInf = BF16 ? 0x7f807f80u : 0x7c007c00u;
-    const uint32_t     a    = v & 0x7fff7fffu;
-    return __vmaxu2(m, a & ~__vcmpgeu2(a, kInf));
+    m = __vmaxu2(m, v.x & 0x7fff7fffu);
+    m = __vmaxu2(m, v.y & 0x7fff7fffu);
+    m = __vmaxu2(m, v.z & 0x7fff7fffu);
+    return __vmaxu2(m, v.w & 0x7fff7fffu);
+}
+
+// Elements that are not finite, as zeros.
+template<bool BF16>
+__device__ __forceinline__ uint32_t finite_only(uint32_t v)
+{
+    return v & ~__vcmpgeu2(v & 0x7fff7fffu, kInfPair<BF16>);
+}
+template<bool BF16>
+__device__ __forceinline__ uint4 finite_only(uint4 v)
+{
+    return make_uint4(finite_only<BF16>(v.x), finite_only<BF16>(v.y), finite_only<BF16>(v.z), finite_only<BF16>(v.w));
 }
 
 template<bool BF16>
-__device__ __forceinline__ float scale_of(uint32_t amax_pair)
+__device__ __forceinline__ float scale_of(uint32_t amax16)
 {
-    const uint32_t a = max(amax_pair & 0xffffu, amax_pair >> 16);
-    return fmaxf(__fdiv_rn(element<BF16>(a), kE4m3Max), kScaleMin);
+    return fmaxf(__fdiv_rn(element<BF16>(amax16), kE4m3Max), kScaleMin);
 }
 
 __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi)
@@ -76,23 +95,21 @@ __device__ __forceinline__ float quotient_for_rounding(float x, float s)
 }
 
 // Whether the rounding of y, an approximation of the quotient within two units in the last place, may differ from the
-// rounding of the quotient itself: y is within four units of a midpoint, or so small that the midpoints lie elsewhere
-// (below 2^-11 everything rounds to zero), or beyond 448 (infinite and NaN elements).
+// rounding of the quotient itself: y is within four units of a midpoint, i.e. its 20 bits below those e4m3 keeps are near
+// 10...0.  Below 2^-6 e4m3 is evenly spaced, as fp32 is between 2^-6 and 2^-5 cut to three bits, so y is looked at there.
 __device__ __forceinline__ bool doubtful(float y)
 {
-    const uint32_t a    = __float_as_uint(y) & 0x7fffffffu;
-    const bool     mid  = ((a & 0xfffffu) - 0x7fffcu) <= 8u;
-    const bool     tiny = (a - 0x3a000000u) < (0x3c800000u - 0x3a000000u);  // [2^-11, 2^-6)
-    return mid || tiny || a > 0x43e00010u;
+    float t = fabsf(y);
+    t       = t < 0.015625f ? t + 0.015625f : t;
+    return (__float_as_uint(t) << 12) - (0x7fffcu << 12) <= (8u << 12);
 }
 
-// Eight elements (one 16-byte load) to eight codes.
+// Eight elements (one 16-byte load) to eight codes.  redo: the block holds elements that are not finite.
 template<bool BF16>
-__device__ __forceinline__ uint2 encode8(uint4 v, float s, float inv)
+__device__ __forceinline__ uint2 encode8(uint4 v, float s, float inv, bool redo)
 {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     float          y[8];
-    bool           redo = false;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         y[2 * i]     = element<BF16>(w[i] & 0xffffu) * inv;
@@ -116,14 +133,14 @@ template<bool BF16>
 __global__ void __launch_bounds__(256)
 quantize_rows_kernel(const uint4* __restrict__ x, uint2* __restrict__ codes, float* __restrict__ scales, int rows, int cols, int kb)
 {
-    __shared__ float   tile[8][9];
-    const int          warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int          kb_groups = (kb + 7) / 8;
-    const int          row0     = static_cast<int>(blockIdx.x / kb_groups) * 8;
-    const int          row      = row0 + warp;
-    const int          kb0      = static_cast<int>(blockIdx.x % kb_groups) * 8;
-    const int          per_row  = cols / 8;
-    const int          first    = kb0 * (kBlock / 8) + lane;
+    __shared__ float tile[8][9];
+    const int        warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int        kb_groups = (kb + 7) / 8;
+    const int        row0      = static_cast<int>(blockIdx.x / kb_groups) * 8;
+    const int        row       = row0 + warp;
+    const int        kb0       = static_cast<int>(blockIdx.x % kb_groups) * 8;
+    const int        per_row   = cols / 8;
+    const int        first     = kb0 * (kBlock / 8) + lane;
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
     if (row < rows) {
@@ -132,19 +149,41 @@ quantize_rows_kernel(const uint4* __restrict__ x, uint2* __restrict__ codes, flo
 #pragma unroll
         for (int i = 0; i < 4; i++)
             v[i] = first + 32 * i < per_row ? ptx::ld_stream_128(x + base + first + 32 * i) : make_uint4(0, 0, 0, 0);
+        // amax of this half-warp's four blocks, two blocks to a register
+        auto amax_of = [&](bool only_finite, uint32_t* pair) {
+            uint32_t m[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                m[i] = amax_bits(0u, only_finite ? finite_only<BF16>(v[i]) : v[i]);
+                m[i] = max(m[i] & 0xffffu, m[i] >> 16);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                pair[i] = m[2 * i] | (m[2 * i + 1] << 16);
+#pragma unroll
+                for (int d = 8; d > 0; d >>= 1)
+                    pair[i] = __vmaxu2(pair[i], __shfl_xor_sync(0xffffffffu, pair[i], d));
+            }
+        };
+        uint32_t pair[2];
+        amax_of(false, pair);
+        const uint32_t most = __vmaxu2(pair[0], pair[1]);
+        const bool     redo = __any_sync(0xffffffffu, max(most & 0xffffu, most >> 16) >= (kInfPair<BF16> & 0xffffu));
+        if (redo)
+            amax_of(true, pair);
+        // lane i of a half computes block i's scale and its reciprocal for the others
+        const uint32_t mine  = (lane & 2) ? pair[1] : pair[0];
+        const float    scale = scale_of<BF16>((lane & 1) ? mine >> 16 : mine & 0xffffu);
+        const float    recip = __frcp_rn(scale);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            uint32_t m = amax_bits<BF16>(amax_bits<BF16>(amax_bits<BF16>(amax_bits<BF16>(0u, v[i].x), v[i].y), v[i].z), v[i].w);
-#pragma unroll
-            for (int d = 8; d > 0; d >>= 1)
-                m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, d));
-            const float s   = scale_of<BF16>(m);
-            const float inv = __frcp_rn(s);
+            const float s   = __shfl_sync(0xffffffffu, scale, i, 16);
+            const float inv = __shfl_sync(0xffffffffu, recip, i, 16);
             if (first + 32 * i < per_row)
-                codes[base + first + 32 * i] = encode8<BF16>(v[i], s, inv);
-            if ((lane & 15) == 0)
-                tile[2 * i + (lane >> 4)][warp] = s;
+                codes[base + first + 32 * i] = encode8<BF16>(v[i], s, inv, redo);
         }
+        if ((lane & 15) < 4)
+            tile[2 * (lane & 3) + (lane >> 4)][warp] = scale;
     }
     __syncthreads();
     const int k = threadIdx.x >> 3, r = threadIdx.x & 7;
@@ -170,29 +209,36 @@ quantize_blocks_kernel(const uint4* __restrict__ x, uint2* __restrict__ codes, f
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
     uint4    v[8];
-    uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < 8; i++)
         v[i] = col < per_row && row0 + 16 * i < rows ? ptx::ld_stream_128(x + base + static_cast<size_t>(row0 + 16 * i) * per_row)
                                                      : make_uint4(0, 0, 0, 0);
+    auto amax_of = [&](bool only_finite) {
+        uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-        m = amax_bits<BF16>(amax_bits<BF16>(amax_bits<BF16>(amax_bits<BF16>(m, v[i].x), v[i].y), v[i].z), v[i].w);
+        for (int i = 0; i < 8; i++)
+            m = amax_bits(m, only_finite ? finite_only<BF16>(v[i]) : v[i]);
+        m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
+        if ((threadIdx.x & 31) == 0)
+            warp_max[threadIdx.x >> 5] = m;
+        __syncthreads();
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1)
-        m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, d));
-    if ((threadIdx.x & 31) == 0)
-        warp_max[threadIdx.x >> 5] = m;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 8; w++)
-        m = __vmaxu2(m, warp_max[w]);
+        for (int w = 0; w < 8; w++)
+            m = max(m, warp_max[w]);
+        return m;
+    };
+    uint32_t   m    = amax_of(false);
+    const bool redo = m >= (kInfPair<BF16> & 0xffffu);
+    if (redo) {
+        __syncthreads();
+        m = amax_of(true);
+    }
     const float s   = scale_of<BF16>(m);
     const float inv = __frcp_rn(s);
 #pragma unroll
     for (int i = 0; i < 8; i++)
         if (col < per_row && row0 + 16 * i < rows)
-            codes[base + static_cast<size_t>(row0 + 16 * i) * per_row] = encode8<BF16>(v[i], s, inv);
+            codes[base + static_cast<size_t>(row0 + 16 * i) * per_row] = encode8<BF16>(v[i], s, inv, redo);
     if (threadIdx.x == 0)
         scales[blockIdx.x] = s;
 }
