@@ -8,16 +8,16 @@
 // quotient clear of fp32's subnormals.  e4m3 has no infinity: an element that is infinite or NaN becomes NaN, which
 // reaches every result that uses it, and its neighbours in the block are scaled as if it were not there.
 //
-// Rounding to the nearest value of the *exact* quotient: x * (1 / s) is off by at most two units in the last place of
-// fp32, so the rounding of that product can differ from the rounding of the quotient only where the product lies within
-// a few units of the midpoint between two e4m3 values.  Those elements (about one in 10^5) take the slow path: the
-// correctly rounded quotient, and where the remainder is not zero a step of one unit towards the exact quotient if that
-// makes the last bit odd -- a midpoint is a number of five bits and never odd, so the second rounding then sees the right
-// side.
+// Rounding to the nearest value of the *exact* quotient: x is multiplied by a number a little below 1 / s and by one a
+// little above, so that the exact quotient lies between the two products.  Rounding never changes the order of two numbers:
+// where both products get the same code, the quotient has it too.  Otherwise the quotient is next to the midpoint m of the
+// two codes' values, and x - m * s, whose sign one fused multiply-add gives exactly, says on which side.  That is no rare
+// case: two bf16 numbers of eight bits often have a ratio that is a midpoint but for the rounding of s (one element in 200;
+// fp16: one in 1500), so it has to be cheap as well: it costs about eight instructions per element of a lane that needs it.
 //
-// Bound by memory (2 bytes in, 1 out per element) once an element costs about ten instructions.  Dividing every element,
-// or sending the ones below the smallest normal e4m3 value down the slow path (a few per cent of them where some features
-// are much larger than others, so nearly every warp), made it twice as slow.
+// Bound by memory (2 bytes in, 1 out per element) only if an element costs less than about ten instructions.  Dividing, or
+// looking at the product's bits for the neighbourhood of a midpoint (and differently below the smallest normal e4m3 value),
+// costs two to three times that; 16 elements per lane halve the shuffles and index arithmetic of 8.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -81,57 +81,69 @@ __device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi)
     return out;
 }
 
-// The quotient x / s as an fp32 number that rounds to e4m3 as the exact quotient does.
-__device__ __forceinline__ float quotient_for_rounding(float x, float s)
+// A block's scale, and the factors a little below and above 1 / scale.
+struct BlockScale {
+    float scale, below, above;
+};
+
+__device__ __forceinline__ BlockScale block_scale(float scale)
 {
-    const float q = __fdiv_rn(x, s);
-    if (!(fabsf(x) <= 3.4028234663852886e38f))
-        return __int_as_float(0x7fffffff);  // infinite or NaN
-    const float r = __fmaf_rn(-q, s, x);  // exact
-    int         b = __float_as_int(q);
-    if (r != 0.0f && (b & 1) == 0)
-        b += ((__float_as_int(r) ^ b) >= 0) ? 1 : -1;
-    return __int_as_float(b);
+    // 1 / scale is off by half a unit in the last place, a product with it by another half: two units more or less bound both
+    const int inv = __float_as_int(__frcp_rn(scale));
+    return BlockScale{scale, __int_as_float(inv - 2), __int_as_float(inv + 2)};
 }
 
-// Whether the rounding of y, an approximation of the quotient within two units in the last place, may differ from the
-// rounding of the quotient itself: y is within four units of a midpoint, i.e. its 20 bits below those e4m3 keeps are near
-// 10...0.  Below 2^-6 e4m3 is evenly spaced, as fp32 is between 2^-6 and 2^-5 cut to three bits, so y is looked at there.
-__device__ __forceinline__ bool doubtful(float y)
+// The codes of two quotients x / s that lie between the values of `lo` and `hi` (neighbours, or the same).
+__device__ __forceinline__ uint32_t settle(uint32_t lo, uint32_t hi, float x0, float x1, float s)
 {
-    float t = fabsf(y);
-    t       = t < 0.015625f ? t + 0.015625f : t;
-    return (__float_as_uint(t) << 12) - (0x7fffcu << 12) <= (8u << 12);
+    uint32_t a, b;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(a) : "h"(static_cast<uint16_t>(lo)));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(b) : "h"(static_cast<uint16_t>(hi)));
+    const float2 sum = __half22float2(__hadd2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b)));
+    const float  r0 = __fmaf_rn(-0.5f * sum.x, s, x0), r1 = __fmaf_rn(-0.5f * sum.y, s, x1);
+    const bool   far0 = r0 == 0.0f ? (hi & 1u) == 0 : (__float_as_int(r0) ^ __float_as_int(x0)) >= 0;
+    const bool   far1 = r1 == 0.0f ? (hi & 0x100u) == 0 : (__float_as_int(r1) ^ __float_as_int(x1)) >= 0;
+    const uint32_t take = (far0 ? 0x00ffu : 0u) | (far1 ? 0xff00u : 0u);
+    return (hi & take) | (lo & ~take);
 }
 
-// Eight elements (one 16-byte load) to eight codes.  redo: the block holds elements that are not finite.
+// Eight elements to eight codes.  redo: the block holds elements that are not finite (all their bits set they are NaN).
 template<bool BF16>
-__device__ __forceinline__ uint2 encode8(uint4 v, float s, float inv, bool redo)
+__device__ __forceinline__ uint2 encode8(uint4 v, BlockScale s, bool redo)
 {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    float          y[8];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        y[2 * i]     = element<BF16>(w[i] & 0xffffu) * inv;
-        y[2 * i + 1] = element<BF16>(w[i] >> 16) * inv;
-        redo |= doubtful(y[2 * i]) | doubtful(y[2 * i + 1]);
-    }
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
     if (redo) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            y[2 * i]     = quotient_for_rounding(element<BF16>(w[i] & 0xffffu), s);
-            y[2 * i + 1] = quotient_for_rounding(element<BF16>(w[i] >> 16), s);
-        }
+        for (int i = 0; i < 4; i++)
+            w[i] |= __vcmpgeu2(w[i] & 0x7fff7fffu, kInfPair<BF16>);
     }
-    return make_uint2(e4m3_pair(y[0], y[1]) | (e4m3_pair(y[2], y[3]) << 16), e4m3_pair(y[4], y[5]) | (e4m3_pair(y[6], y[7]) << 16));
+    uint32_t lo[4], hi[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float x0 = element<BF16>(w[i] & 0xffffu), x1 = element<BF16>(w[i] >> 16);
+        lo[i] = e4m3_pair(x0 * s.below, x1 * s.below);
+        hi[i] = e4m3_pair(x0 * s.above, x1 * s.above);
+    }
+    if ((lo[0] | (lo[1] << 16)) != (hi[0] | (hi[1] << 16)) || (lo[2] | (lo[3] << 16)) != (hi[2] | (hi[3] << 16))) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            lo[i] = settle(lo[i], hi[i], element<BF16>(w[i] & 0xffffu), element<BF16>(w[i] >> 16), s.scale);
+    }
+    return make_uint2(lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16));
 }
 
-// Blocks of 1 x 128.  A thread block takes 8 rows (one per warp) x 8 blocks of columns: a half-warp holds a block (16
-// bytes per lane), so a warp reads 512 contiguous bytes per load and has four of them in flight, and the 64 scales go
-// out through shared memory as runs of eight consecutive tokens.
+template<bool BF16>
+__device__ __forceinline__ uint4 encode16(const uint4* v, BlockScale s, bool redo)
+{
+    const uint2 a = encode8<BF16>(v[0], s, redo), b = encode8<BF16>(v[1], s, redo);
+    return make_uint4(a.x, a.y, b.x, b.y);
+}
+
+// Blocks of 1 x 128.  A thread block takes 8 rows (one per warp) x 8 blocks of columns: eight lanes hold a block (two 16-byte
+// loads each), a warp has 2 KB in flight, and the 64 scales go out through shared memory as runs of eight consecutive tokens.
 template<bool BF16>
 __global__ void __launch_bounds__(256)
-quantize_rows_kernel(const uint4* __restrict__ x, uint2* __restrict__ codes, float* __restrict__ scales, int rows, int cols, int kb)
+quantize_rows_kernel(const uint4* __restrict__ x, uint4* __restrict__ codes, float* __restrict__ scales, int rows, int cols, int kb)
 {
     __shared__ float tile[8][9];
     const int        warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -139,51 +151,49 @@ quantize_rows_kernel(const uint4* __restrict__ x, uint2* __restrict__ codes, flo
     const int        row0      = static_cast<int>(blockIdx.x / kb_groups) * 8;
     const int        row       = row0 + warp;
     const int        kb0       = static_cast<int>(blockIdx.x % kb_groups) * 8;
-    const int        per_row   = cols / 8;
-    const int        first     = kb0 * (kBlock / 8) + lane;
+    const int        per_row   = cols / 16;  // lanes' worth of elements
+    const int        first     = kb0 * (kBlock / 16) + lane;
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
     if (row < rows) {
-        const size_t base = static_cast<size_t>(row) * per_row;
-        uint4        v[4];
+        const size_t base = static_cast<size_t>(row) * per_row + first;
+        uint4        v[2][2];  // blocks kb0 + lane / 8 and that + 4
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            v[i] = first + 32 * i < per_row ? ptx::ld_stream_128(x + base + first + 32 * i) : make_uint4(0, 0, 0, 0);
-        // amax of this half-warp's four blocks, two blocks to a register
-        auto amax_of = [&](bool only_finite, uint32_t* pair) {
-            uint32_t m[4];
+        for (int i = 0; i < 2; i++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                m[i] = amax_bits(0u, only_finite ? finite_only<BF16>(v[i]) : v[i]);
-                m[i] = max(m[i] & 0xffffu, m[i] >> 16);
-            }
+            for (int h = 0; h < 2; h++)
+                v[i][h] = first + 32 * i < per_row ? ptx::ld_stream_128(x + 2 * (base + 32 * i) + h) : make_uint4(0, 0, 0, 0);
+        // amax of the lane's two blocks, one per half of a register
+        auto amax_of = [&](bool only_finite) {
+            uint32_t m[2];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                pair[i] = m[2 * i] | (m[2 * i + 1] << 16);
-#pragma unroll
-                for (int d = 8; d > 0; d >>= 1)
-                    pair[i] = __vmaxu2(pair[i], __shfl_xor_sync(0xffffffffu, pair[i], d));
+                m[i] = only_finite ? amax_bits(amax_bits(0u, finite_only<BF16>(v[i][0])), finite_only<BF16>(v[i][1]))
+                                   : amax_bits(amax_bits(0u, v[i][0]), v[i][1]);
+                m[i] = max(m[i] & 0xffffu, m[i] >> 16);
             }
-        };
-        uint32_t pair[2];
-        amax_of(false, pair);
-        const uint32_t most = __vmaxu2(pair[0], pair[1]);
-        const bool     redo = __any_sync(0xffffffffu, max(most & 0xffffu, most >> 16) >= (kInfPair<BF16> & 0xffffu));
-        if (redo)
-            amax_of(true, pair);
-        // lane i of a half computes block i's scale and its reciprocal for the others
-        const uint32_t mine  = (lane & 2) ? pair[1] : pair[0];
-        const float    scale = scale_of<BF16>((lane & 1) ? mine >> 16 : mine & 0xffffu);
-        const float    recip = __frcp_rn(scale);
+            uint32_t pair = m[0] | (m[1] << 16);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float s   = __shfl_sync(0xffffffffu, scale, i, 16);
-            const float inv = __shfl_sync(0xffffffffu, recip, i, 16);
+            for (int d = 4; d > 0; d >>= 1)
+                pair = __vmaxu2(pair, __shfl_xor_sync(0xffffffffu, pair, d));
+            return pair;
+        };
+        uint32_t   pair = amax_of(false);
+        const bool redo = __any_sync(0xffffffffu, max(pair & 0xffffu, pair >> 16) >= (kInfPair<BF16> & 0xffffu));
+        if (redo)
+            pair = amax_of(true);
+        // even lanes work out the first block's scale, odd ones the second's
+        const float scale = scale_of<BF16>((lane & 1) ? pair >> 16 : pair & 0xffffu);
+        const BlockScale mine = block_scale(scale);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const BlockScale s{__shfl_sync(0xffffffffu, mine.scale, i, 8), __shfl_sync(0xffffffffu, mine.below, i, 8),
+                               __shfl_sync(0xffffffffu, mine.above, i, 8)};
             if (first + 32 * i < per_row)
-                codes[base + first + 32 * i] = encode8<BF16>(v[i], s, inv, redo);
+                codes[base + 32 * i] = encode16<BF16>(v[i], s, redo);
         }
-        if ((lane & 15) < 4)
-            tile[2 * (lane & 3) + (lane >> 4)][warp] = scale;
+        if ((lane & 7) < 2)
+            tile[4 * (lane & 1) + (lane >> 3)][warp] = scale;
     }
     __syncthreads();
     const int k = threadIdx.x >> 3, r = threadIdx.x & 7;
@@ -191,33 +201,35 @@ quantize_rows_kernel(const uint4* __restrict__ x, uint2* __restrict__ codes, flo
         scales[static_cast<size_t>(kb0 + k) * rows + row0 + r] = tile[k][r];
 }
 
-// Blocks of 128 x 128, one per thread block: 16 lanes per row, 16 rows per pass, the whole block (32 KB) in registers
+// Blocks of 128 x 128, one per thread block: 8 lanes per row, 32 rows per pass, the whole block (32 KB) in registers
 // between the one read and the one write.
 template<bool BF16>
 __global__ void __launch_bounds__(256)
-quantize_blocks_kernel(const uint4* __restrict__ x, uint2* __restrict__ codes, float* __restrict__ scales, int rows, int cols, int kb,
+quantize_blocks_kernel(const uint4* __restrict__ x, uint4* __restrict__ codes, float* __restrict__ scales, int rows, int cols, int kb,
                        int row_blocks)
 {
     __shared__ uint32_t warp_max[8];
     const int           kblock = static_cast<int>(blockIdx.x % kb);
     const int           rblock = static_cast<int>(blockIdx.x / kb) % row_blocks;
     const size_t        group  = blockIdx.x / (static_cast<unsigned>(kb) * row_blocks);
-    const int           col    = kblock * (kBlock / 8) + (threadIdx.x & 15);
-    const int           row0   = rblock * kBlock + static_cast<int>(threadIdx.x >> 4);
-    const int           per_row = cols / 8;
-    const size_t        base    = group * rows * static_cast<size_t>(per_row) + col;
+    const int           col    = kblock * (kBlock / 16) + (threadIdx.x & 7);
+    const int           row0   = rblock * kBlock + static_cast<int>(threadIdx.x >> 3);
+    const int           per_row = cols / 16;
+    const size_t        base    = (group * rows + row0) * per_row + col;
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
-    uint4    v[8];
+    uint4 v[4][2];
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-        v[i] = col < per_row && row0 + 16 * i < rows ? ptx::ld_stream_128(x + base + static_cast<size_t>(row0 + 16 * i) * per_row)
-                                                     : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+            v[i][h] = col < per_row && row0 + 32 * i < rows ? ptx::ld_stream_128(x + 2 * (base + static_cast<size_t>(32 * i) * per_row) + h)
+                                                            : make_uint4(0, 0, 0, 0);
     auto amax_of = [&](bool only_finite) {
         uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            m = amax_bits(m, only_finite ? finite_only<BF16>(v[i]) : v[i]);
+            m = amax_bits(m, only_finite ? finite_only<BF16>(v[i / 2][i % 2]) : v[i / 2][i % 2]);
         m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
         if ((threadIdx.x & 31) == 0)
             warp_max[threadIdx.x >> 5] = m;
@@ -233,14 +245,13 @@ quantize_blocks_kernel(const uint4* __restrict__ x, uint2* __restrict__ codes, f
         __syncthreads();
         m = amax_of(true);
     }
-    const float s   = scale_of<BF16>(m);
-    const float inv = __frcp_rn(s);
+    const BlockScale s = block_scale(scale_of<BF16>(m));
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-        if (col < per_row && row0 + 16 * i < rows)
-            codes[base + static_cast<size_t>(row0 + 16 * i) * per_row] = encode8<BF16>(v[i], s, inv, redo);
+    for (int i = 0; i < 4; i++)
+        if (col < per_row && row0 + 32 * i < rows)
+            codes[base + static_cast<size_t>(32 * i) * per_row] = encode16<BF16>(v[i], s, redo);
     if (threadIdx.x == 0)
-        scales[blockIdx.x] = s;
+        scales[blockIdx.x] = s.scale;
 }
 
 template<typename... P, typename... Args>
@@ -282,7 +293,7 @@ extern "C" int spmm_b200_quantize_fp8(
             return static_cast<int>(cudaErrorInvalidValue);
         auto kern = X_type == SPMM_B200_BF16 ? quantize_rows_kernel<true> : quantize_rows_kernel<false>;
         return static_cast<int>(launch(st, kern, dim3(static_cast<unsigned>(blocks)), static_cast<const uint4*>(X),
-                                       static_cast<uint2*>(codes), scales, rows, cols, kb));
+                                       static_cast<uint4*>(codes), scales, rows, cols, kb));
     }
     const int  row_blocks = (rows - 1) / kBlock + 1;
     const long blocks     = static_cast<long>(groups) * row_blocks * kb;
@@ -290,5 +301,5 @@ extern "C" int spmm_b200_quantize_fp8(
         return static_cast<int>(cudaErrorInvalidValue);
     auto kern = X_type == SPMM_B200_BF16 ? quantize_blocks_kernel<true> : quantize_blocks_kernel<false>;
     return static_cast<int>(launch(st, kern, dim3(static_cast<unsigned>(blocks)), static_cast<const uint4*>(X),
-                                   static_cast<uint2*>(codes), scales, rows, cols, kb, row_blocks));
+                                   static_cast<uint4*>(codes), scales, rows, cols, kb, row_blocks));
 }
