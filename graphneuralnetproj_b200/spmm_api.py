@@ -272,42 +272,53 @@ def spmm_own_scratch(stream, Compressed_A, TileOffsets, B, C, M_Global, N_Global
                                           _dev_ptr(B), _dev_ptr(C), M_Global, N_Global, K_Global)
 
 
-def _operands(stream, *operands):
-    """(stream handle, [device pointers]) after checking each (name, tensor, dtypes, elements): a contiguous CUDA tensor
-    of the stream's device, which is the current one, of one of the types and with exactly that many elements."""
-    import torch
-    device = torch.cuda.current_device()
+class _Torch:
+    """What the linear layers need of torch, looked up at their first call (the host functions do without torch)."""
+    ready = False
+
+    @classmethod
+    def load(cls):
+        import torch
+        cls.halves = (torch.float16, torch.bfloat16)
+        cls.bf16 = torch.bfloat16
+        cls.codes = (torch.float8_e4m3fn, torch.uint8)
+        cls.single = (torch.float32,)
+        cls.index = (torch.int32,)
+        cls.current_device = torch.cuda.current_device
+        cls.current_stream = torch.cuda.current_stream
+        # the handle alone, without a Stream object around it, where this torch has it
+        cls.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+        cls.ready = True
+
+
+def _launch_on(stream):
+    """(current device, stream handle) for a call on `stream`: None, a raw handle, or a torch.cuda.Stream of that device."""
+    if not _Torch.ready:
+        _Torch.load()
+    device = _Torch.current_device()
     if stream is None:
-        stream = torch.cuda.current_stream()
-    if not isinstance(stream, int):
-        if stream.device.index != device:
-            raise ValueError("the stream belongs to device %s, the current device is %d" % (stream.device, device))
-        stream = stream.cuda_stream
-    pointers = []
-    for name, t, dtypes, elements in operands:
-        if not t.is_cuda or t.get_device() != device:
-            raise ValueError("%s must be a CUDA tensor on the current device" % name)
-        if t.dtype not in dtypes:
-            raise ValueError("%s has type %s, expected one of %s" % (name, t.dtype, ", ".join(map(str, dtypes))))
-        if t.numel() != elements:
-            raise ValueError("%s has %d elements, expected %d" % (name, t.numel(), elements))
-        if not t.is_contiguous():
-            raise ValueError("%s must be contiguous" % name)
-        pointers.append(t.data_ptr())
-    return stream, pointers
+        return device, _Torch.raw_stream(device)
+    if isinstance(stream, int):
+        return device, stream
+    if stream.device.index != device:
+        raise ValueError("the stream belongs to device %s, the current device is %d" % (stream.device, device))
+    return device, stream.cuda_stream
 
 
-def _types():
-    import torch
-    return (torch.float16, torch.bfloat16), (torch.float8_e4m3fn, torch.uint8), (torch.float32,), (torch.int32,)
+def _operand(name, t, device, dtypes, elements):
+    """The address of a contiguous tensor on the current device, of one of the types and with exactly that many elements."""
+    if t.get_device() != device or t.dtype not in dtypes or t.numel() != elements or not t.is_contiguous():
+        raise ValueError("%s must be a contiguous tensor of %d elements on CUDA device %d, of type %s; got %s of type %s on %s%s"
+                         % (name, elements, device, " or ".join(map(str, dtypes)), tuple(t.shape), t.dtype, t.device,
+                            "" if t.is_contiguous() else ", not contiguous"))
+    return t.data_ptr()
 
 
-def _workspace(workspace):
-    """(pointer, bytes) of a workspace tensor, or of none."""
+def _workspace(workspace, device):
+    """(address, bytes) of a workspace tensor, or of none."""
     if workspace is None:
         return None, 0
-    import torch
-    if not workspace.is_contiguous() or not workspace.is_cuda or workspace.get_device() != torch.cuda.current_device():
+    if workspace.get_device() != device or not workspace.is_contiguous():
         raise ValueError("the workspace must be a contiguous CUDA tensor on the current device")
     return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
@@ -322,14 +333,16 @@ def quantize_fp8(stream, X, codes, scales, block_rows):
     block_rows = 1: one scale per 1 x 128 block, scales[ceil(cols / 128)][rows] (activations); block_rows = 128: one per
     128 x 128 block, scales[(groups)][ceil(rows / 128)][ceil(cols / 128)] (weights).  codes: float8_e4m3fn or uint8, the
     shape of X.  See spmm_b200_quantize_fp8 in include/spmm_b200.h for the rounding.  Returns a cudaError_t as an int."""
-    wide, eight, single, _ = _types()
     if X.dim() not in (2, 3) or block_rows not in (1, 128) or (block_rows == 1 and X.dim() != 2):
         raise ValueError("X must be [rows][cols], or [groups][rows][cols] with block_rows = 128; block_rows 1 or 128")
     groups = X.shape[0] if X.dim() == 3 else 1
     rows, cols = X.shape[-2:]
     blocks = _blocks(cols) * (rows if block_rows == 1 else groups * _blocks(rows))
-    handle, (x, c, s) = _operands(stream, ("X", X, wide, X.numel()), ("codes", codes, eight, X.numel()), ("scales", scales, single, blocks))
-    return LIB.spmm_b200_quantize_fp8(handle, x, int(X.dtype is wide[1]), groups, rows, cols, block_rows, c, s)
+    device, handle = _launch_on(stream)
+    elements = X.numel()
+    return LIB.spmm_b200_quantize_fp8(handle, _operand("X", X, device, _Torch.halves, elements), int(X.dtype is _Torch.bf16), groups, rows, cols,
+                                      block_rows, _operand("codes", codes, device, _Torch.codes, elements),
+                                      _operand("scales", scales, device, _Torch.single, blocks))
 
 
 def linear_workspace_bytes(groups, M_Global, N_Global, K_Global, eight_bit):
@@ -341,39 +354,44 @@ def fp8_linear(stream, A, A_scales, B, B_scales, C, M_Global, N_Global, K_Global
     """C[N][M] = B[N][K] * A[M][K]^T from e4m3 codes and the scales quantize_fp8 gives (weights: block_rows = 128,
     activations: block_rows = 1); C fp16 or bf16.  workspace: a CUDA tensor, zero-filled once, of
     linear_workspace_bytes(1, M, N, K, True) bytes, or None.  Returns a cudaError_t as an int; asynchronous."""
-    wide, eight, single, _ = _types()
     M, N, K = M_Global, N_Global, K_Global
-    handle, (a, sa, b, sb, c) = _operands(stream, ("A", A, eight, M * K), ("A_scales", A_scales, single, _blocks(M) * _blocks(K)),
-                                          ("B", B, eight, N * K), ("B_scales", B_scales, single, _blocks(K) * N), ("C", C, wide, N * M))
-    ws, ws_bytes = _workspace(workspace)
-    return LIB.spmm_b200_fp8_linear(handle, a, sa, b, sb, c, int(C.dtype is wide[1]), M, N, K, ws, ws_bytes)
+    device, handle = _launch_on(stream)
+    ws, ws_bytes = _workspace(workspace, device)
+    return LIB.spmm_b200_fp8_linear(handle, _operand("A", A, device, _Torch.codes, M * K),
+                                    _operand("A_scales", A_scales, device, _Torch.single, _blocks(M) * _blocks(K)),
+                                    _operand("B", B, device, _Torch.codes, N * K),
+                                    _operand("B_scales", B_scales, device, _Torch.single, _blocks(K) * N),
+                                    _operand("C", C, device, _Torch.halves, N * M), int(C.dtype is _Torch.bf16), M, N, K, ws, ws_bytes)
 
 
 def grouped_linear(stream, A, B, C, group_offsets, groups, M_Global, N_Global, K_Global, workspace):
     """C[t] = B[t] * A[g]^T for the tokens t of group g, group_offsets[g] <= t < group_offsets[g + 1] (int32, on the
     device); A[groups][M][K], B[N][K], C[N][M], all fp16 or all bf16.  Rows of C outside all groups stay as they were.
     workspace: linear_workspace_bytes(groups, M, N, K, False) bytes, zero-filled once, or None."""
-    wide, _, _, index = _types()
     M, N, K = M_Global, N_Global, K_Global
     if B.dtype is not A.dtype or C.dtype is not A.dtype:
         raise ValueError("A, B and C must have the same type")
-    handle, (a, b, c, o) = _operands(stream, ("A", A, wide, groups * M * K), ("B", B, wide, N * K), ("C", C, wide, N * M),
-                                     ("group_offsets", group_offsets, index, groups + 1))
-    ws, ws_bytes = _workspace(workspace)
-    return LIB.spmm_b200_grouped_linear(handle, a, b, c, int(C.dtype is wide[1]), o, groups, M, N, K, ws, ws_bytes)
+    device, handle = _launch_on(stream)
+    ws, ws_bytes = _workspace(workspace, device)
+    return LIB.spmm_b200_grouped_linear(handle, _operand("A", A, device, _Torch.halves, groups * M * K),
+                                        _operand("B", B, device, _Torch.halves, N * K), _operand("C", C, device, _Torch.halves, N * M),
+                                        int(C.dtype is _Torch.bf16),
+                                        _operand("group_offsets", group_offsets, device, _Torch.index, groups + 1), groups, M, N, K, ws, ws_bytes)
 
 
 def grouped_fp8_linear(stream, A, A_scales, B, B_scales, C, group_offsets, groups, M_Global, N_Global, K_Global, workspace):
     """grouped_linear from e4m3 codes and scales: A[groups][M][K] with A_scales[groups][ceil(M / 128)][ceil(K / 128)],
     B[N][K] with B_scales[ceil(K / 128)][N]; C fp16 or bf16."""
-    wide, eight, single, index = _types()
     M, N, K = M_Global, N_Global, K_Global
-    handle, (a, sa, b, sb, c, o) = _operands(
-        stream, ("A", A, eight, groups * M * K), ("A_scales", A_scales, single, groups * _blocks(M) * _blocks(K)),
-        ("B", B, eight, N * K), ("B_scales", B_scales, single, _blocks(K) * N), ("C", C, wide, N * M),
-        ("group_offsets", group_offsets, index, groups + 1))
-    ws, ws_bytes = _workspace(workspace)
-    return LIB.spmm_b200_grouped_fp8_linear(handle, a, sa, b, sb, c, int(C.dtype is wide[1]), o, groups, M, N, K, ws, ws_bytes)
+    device, handle = _launch_on(stream)
+    ws, ws_bytes = _workspace(workspace, device)
+    return LIB.spmm_b200_grouped_fp8_linear(handle, _operand("A", A, device, _Torch.codes, groups * M * K),
+                                            _operand("A_scales", A_scales, device, _Torch.single, groups * _blocks(M) * _blocks(K)),
+                                            _operand("B", B, device, _Torch.codes, N * K),
+                                            _operand("B_scales", B_scales, device, _Torch.single, _blocks(K) * N),
+                                            _operand("C", C, device, _Torch.halves, N * M), int(C.dtype is _Torch.bf16),
+                                            _operand("group_offsets", group_offsets, device, _Torch.index, groups + 1), groups, M, N, K,
+                                            ws, ws_bytes)
 
 
 def linear_plan(tiles, kb, workers, overhead):
