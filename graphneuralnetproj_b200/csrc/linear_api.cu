@@ -121,7 +121,7 @@ cudaError_t launch(cudaStream_t stream, LinearParams& p, const LinearShape& s)
         return e;
     auto      kern        = PAIR ? linear_pair_kernel<EIGHT> : linear_kernel<EIGHT>;
     const int stage_bytes = PAIR ? kPairStageBytes : kStepBlocks * (kLinearBoxBytes + s.nt * 128);
-    const int fixed       = kLinearFixedSmem + (EIGHT ? (PAIR ? 2 * kPairBatch * 1024 : 2 * kGroupScales * 4) : 0) + s.groups * 12;
+    const int fixed       = kLinearFixedSmem + (EIGHT ? (PAIR ? 2 * kPairBatch * 1024 : 2 * kGroupScales * 4) : 0) + s.groups * kLinearTableWords * 4;
     p.stages              = std::min(PAIR ? kPairStages : kLinearMaxStages, (kMaxDynamicSmem - fixed) / stage_bytes);
     p.steps               = PAIR ? s.kb : (s.kb - 1) / kStepBlocks + 1;
 

@@ -59,7 +59,7 @@ linear_pair_kernel(const __grid_constant__ LinearParams p)
     volatile int*      abort_word = reinterpret_cast<volatile int*>(smem + bar_off + kWords + 4);
     int* const         warp_sums  = reinterpret_cast<int*>(smem + bar_off + kWords + 8);
     int* const         groups_at  = reinterpret_cast<int*>(smem + bar_off + 512);
-    const LinearTable  table{groups_at, groups_at + p.groups, groups_at + 2 * p.groups};
+    const LinearTable  table{groups_at, groups_at + p.groups, groups_at + 2 * p.groups, groups_at + 3 * p.groups};
     static_assert(kWords + 8 + 20 * 4 <= 512, "barrier block");
 
     const int      warp = linear_uniform(static_cast<int>(threadIdx.x >> 5)), lane = threadIdx.x & 31;
@@ -87,14 +87,15 @@ linear_pair_kernel(const __grid_constant__ LinearParams p)
     ptx::grid_dependency_wait();
     const int tiles_m = (p.m - 1) / kPairTile + 1;
     ptx::tc_fence_before_sync();
-    linear_build_table(p, table, warp_sums, kPairTile, tiles_m);
+    constexpr int kGranule = EIGHT ? kPairTile : 32;  // with tokens on the lanes a narrower tile costs no less
+    linear_build_table<!EIGHT>(p, table, warp_sums, kPairTile, kGranule, tiles_m);
     ptx::cluster_sync_all();  // both blocks' barriers exist before anyone arrives on the partner's
     ptx::tc_fence_after_sync();
     const uint32_t        tmem_base = linear_uniform(static_cast<int>(*tmem_slot));
     const int             worker    = static_cast<int>(blockIdx.x >> 1);
     const LinearPartition part = make_linear_partition(table.end[p.groups - 1], p.steps, static_cast<int>(gridDim.x >> 1), p.overhead);
 
-    auto locate = [&](int tile) { return linear_locate(p, table, tile, kPairTile, kPairTile, tiles_m); };
+    auto locate = [&](int tile) { return linear_locate(p, table, tile, kPairTile, kGranule, kPairTile, tiles_m); };
     // columns of the accumulator that are used
     auto columns = [&](const LinearTile& t) { return EIGHT ? kPairTile : (t.rows + 31) & ~31; };
 
