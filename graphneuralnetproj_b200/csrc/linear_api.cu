@@ -64,9 +64,24 @@ int max_workers(const LinearShape& s)
     return s.pair ? kMaxWorkers / 2 : kMaxWorkers;
 }
 
+// When cutting tiles pays (linear_plan.h), from measurements.  Few tokens: a block streams a step (32 KB) in 0.43 us while at
+// most about 90 do; cutting costs 4 us up to 32 tokens (1 token, 4096 x 4096, 32 tiles of 16 steps: 11.5 us whole, 10.2 in four
+// parts; 9216 x 9216, 72 of 36: 20.7 and 25), 7 us up to 64 (64 x 2048 x 4096: 13.9 and 15.5).  Over 64 tokens a step takes as
+// long as its arithmetic, about 1 us (90 x 4096 x 2048, 32 tiles of 8: 12.1 and 15.3; 100 x 7168 x 7168, 56 of 28: 38 and 24.6).
+// Pairs: a piece is 128 KB per block, a k-block 0.57 us (512 x 4096 x 14336, 32 tiles of 112: 60 us whole, 43 in two parts; 200 x
+// 2048 x 2048, 8 of 16: 14.8 and 19.1).
+LinearCutting cutting(const LinearShape& s)
+{
+    if (s.pair)
+        return LinearCutting{14, max_workers(s), 4};
+    if (s.nt <= 64)
+        return LinearCutting{s.nt <= 32 ? 9 : 17, 91, 16};
+    return LinearCutting{8, max_workers(s), 16};
+}
+
 size_t workspace_needed(const LinearShape& s)
 {
-    return kCounterBytes + 2 * static_cast<size_t>(max_workers(s)) * s.slot_bytes;
+    return kCounterBytes + static_cast<size_t>(max_workers(s)) * s.slot_bytes;
 }
 
 // Sizes that the format and the index arithmetic can describe.
@@ -209,12 +224,13 @@ cudaError_t linear(cudaStream_t stream, LinearShape s, const void* A, const floa
     p.nt       = s.nt;
     p.b_box    = s.b_box;
     p.bf16     = C_type == SPMM_B200_BF16;
-    p.overhead = -1;
+    p.cutting  = cutting(s);
     if (workspace && workspace_bytes >= workspace_needed(s)) {
         p.counters = static_cast<unsigned*>(workspace);
         p.slots    = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
-        p.overhead = s.pair ? 16 : 2;
     }
+    else
+        p.cutting.overhead = -1;
     p.wide_c = aligned16(C) && s.m % 8 == 0;
     if (s.pair)
         return s.eight ? launch<true, true>(stream, p, s) : launch<false, true>(stream, p, s);
@@ -326,20 +342,18 @@ int spmm_b200_grouped_fp8_linear(void*        stream,
                                    B, B_scales, C, C_type, group_offsets, workspace, workspace_bytes));
 }
 
-int spmm_b200_linear_plan(int tiles, int kb, int workers, int overhead, int worker, int index, int* segment)
+int spmm_b200_linear_plan(int tiles, int kb, int workers, int overhead, int saturating, int pieces, int worker, int index, int* segment)
 {
     using namespace spmm_b200;
-    if (tiles < 0 || kb < 1 || workers < 1 || worker < 0 || worker >= workers || index < 0 || !segment)
+    if (tiles < 0 || kb < 1 || workers < 1 || saturating < 1 || pieces < 1 || worker < 0 || worker >= workers || index < 0 || !segment)
         return static_cast<int>(cudaErrorInvalidValue);
-    const LinearPartition p = make_linear_partition(tiles, kb, workers, overhead);
+    const LinearPartition p = make_linear_partition(tiles, kb, workers, LinearCutting{overhead, saturating, pieces});
     const LinearSegment   s = linear_segment(p, worker, index);
     segment[0] = s.tile;
     segment[1] = s.kb0;
     segment[2] = s.kb1;
-    segment[3] = s.slot;
-    segment[4] = s.first;
-    segment[5] = s.last;
-    segment[6] = s.tile >= 0 && s.slot >= 0 ? linear_slot_of(p, s, worker) : -1;
+    segment[3] = s.first;
+    segment[4] = s.last;
     return static_cast<int>(cudaSuccess);
 }
 

@@ -63,7 +63,7 @@ struct LinearParams {
     int          stages;
     int          bf16;      // C (and 16-bit operands) are bf16, not fp16
     int          wide_c;    // C takes 16-byte stores: aligned, M a multiple of 8
-    int          overhead;  // see make_linear_partition
+    LinearCutting cutting;
 };
 
 // Which part of the layer a tile is.
@@ -306,15 +306,34 @@ linear_kernel(const __grid_constant__ LinearParams p)
         ptx::tmem_alloc(bar_base + kWords, 512);
         ptx::tmem_relinquish();
     }
+    if (threadIdx.x == 0) {
+        ptx::prefetch_tensor_map(&p.a_map);
+        ptx::prefetch_tensor_map(&p.b_map);
+    }
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
 
     const int tiles_m = (p.m - 1) / kLinearRows + 1;
     ptx::tc_fence_before_sync();
-    linear_build_table<false>(p, table, warp_sums, p.nt, 16, tiles_m);
+    if (p.offsets == nullptr) {
+        // One group: the TMA warp, which set up the barriers, need not wait for the others to start the first loads.
+        if (threadIdx.x == 0) {
+            table.row[0]   = 0;
+            table.rows[0]  = p.n;
+            table.group[0] = 0;
+            table.end[0]   = (p.n + p.nt - 1) / p.nt * tiles_m;
+        }
+        __syncwarp();
+        if (warp == 0)
+            ptx::named_arrive(1, kLinearThreads);
+        else
+            ptx::named_sync(1, kLinearThreads);
+    }
+    else
+        linear_build_table<false>(p, table, warp_sums, p.nt, 16, tiles_m);
     ptx::tc_fence_after_sync();
-    const uint32_t        tmem_base = linear_uniform(static_cast<int>(*tmem_slot));
-    const LinearPartition part      = make_linear_partition(table.end[p.groups - 1], p.steps, static_cast<int>(gridDim.x), p.overhead);
+    const uint32_t        tmem_base = warp == 0 ? 0 : linear_uniform(static_cast<int>(*tmem_slot));
+    const LinearPartition part      = make_linear_partition(table.end[p.groups - 1], p.steps, static_cast<int>(gridDim.x), p.cutting);
     const int             worker    = static_cast<int>(blockIdx.x);
 
     auto locate  = [&](int tile) { return linear_locate(p, table, tile, p.nt, 16, kLinearRows, tiles_m); };
@@ -566,7 +585,7 @@ linear_kernel(const __grid_constant__ LinearParams p)
                         linear_store(p, static_cast<size_t>(t.row0 + token) * p.m + m, v[j]);
                 }
             };
-            if (seg.slot < 0) {
+            if (seg.first == seg.last) {
 #pragma unroll
                 for (int c = 0; c < NCH; c++)
                     if (col_of(c) < n) {
@@ -579,7 +598,7 @@ linear_kernel(const __grid_constant__ LinearParams p)
                 // slots: [columns / 4][128 lanes] float4, so that a warp's accesses are contiguous
                 const size_t  slot4 = static_cast<size_t>(kLinearRows) * p.nt / 4;
                 float4* const slots = reinterpret_cast<float4*>(p.slots) + row;
-                float4* const mine  = slots + seg.slot * slot4;
+                float4* const mine  = slots + worker * slot4;
 #pragma unroll
                 for (int c = 0; c < NCH; c++)
                     if (col_of(c) < n) {
@@ -609,7 +628,7 @@ linear_kernel(const __grid_constant__ LinearParams p)
                                 v[j] = 0.0f;
 #pragma unroll 1
                             for (int w = seg.first; w <= seg.last; w++) {
-                                const float4* from = slots + linear_slot_of(part, seg, w) * slot4 + (col_of(c) / 4) * kLinearRows;
+                                const float4* from = slots + w * slot4 + (col_of(c) / 4) * kLinearRows;
 #pragma unroll
                                 for (int j = 0; j < CH / 4; j++) {
                                     const float4 f = __ldcg(from + j * kLinearRows);

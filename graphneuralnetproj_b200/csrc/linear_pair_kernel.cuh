@@ -83,6 +83,10 @@ linear_pair_kernel(const __grid_constant__ LinearParams p)
         ptx::tmem_alloc_pair(bar_base + kWords, 512);
         ptx::tmem_relinquish_pair();
     }
+    if (threadIdx.x == 0) {
+        ptx::prefetch_tensor_map(&p.a_map);
+        ptx::prefetch_tensor_map(&p.b_map);
+    }
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();
     const int tiles_m = (p.m - 1) / kPairTile + 1;
@@ -93,7 +97,7 @@ linear_pair_kernel(const __grid_constant__ LinearParams p)
     ptx::tc_fence_after_sync();
     const uint32_t        tmem_base = linear_uniform(static_cast<int>(*tmem_slot));
     const int             worker    = static_cast<int>(blockIdx.x >> 1);
-    const LinearPartition part = make_linear_partition(table.end[p.groups - 1], p.steps, static_cast<int>(gridDim.x >> 1), p.overhead);
+    const LinearPartition part = make_linear_partition(table.end[p.groups - 1], p.steps, static_cast<int>(gridDim.x >> 1), p.cutting);
 
     auto locate = [&](int tile) { return linear_locate(p, table, tile, kPairTile, kGranule, kPairTile, tiles_m); };
     // columns of the accumulator that are used
@@ -369,7 +373,7 @@ linear_pair_kernel(const __grid_constant__ LinearParams p)
                     if (col_of(c) + j < t.rows)
                         linear_store(p, static_cast<size_t>(t.row0 + col_of(c) + j) * p.m + m, v[j]);
             };
-            if (seg.slot < 0) {
+            if (seg.first == seg.last) {
 #pragma unroll
                 for (int c = 0; c < NCH; c++)
                     if (col_of(c) < n) {
@@ -381,7 +385,7 @@ linear_pair_kernel(const __grid_constant__ LinearParams p)
             else {
                 constexpr size_t kSlot4 = static_cast<size_t>(kLinearRows) * kPairTile / 4;
                 float4* const    slots  = reinterpret_cast<float4*>(p.slots) + rank * kSlot4 + row;
-                float4* const    mine   = slots + 2 * seg.slot * kSlot4;
+                float4* const    mine   = slots + static_cast<size_t>(2 * worker) * kSlot4;
 #pragma unroll
                 for (int c = 0; c < NCH; c++)
                     if (col_of(c) < n) {
@@ -411,7 +415,7 @@ linear_pair_kernel(const __grid_constant__ LinearParams p)
                                 v[j] = 0.0f;
 #pragma unroll 1
                             for (int w = seg.first; w <= seg.last; w++) {
-                                const float4* from = slots + 2 * linear_slot_of(part, seg, w) * kSlot4 + (col_of(c) / 4) * kLinearRows;
+                                const float4* from = slots + static_cast<size_t>(2 * w) * kSlot4 + (col_of(c) / 4) * kLinearRows;
 #pragma unroll
                                 for (int j = 0; j < CH / 4; j++) {
                                     const float4 f = __ldcg(from + j * kLinearRows);

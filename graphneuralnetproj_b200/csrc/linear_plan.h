@@ -1,14 +1,16 @@
 // How the tiles of a linear layer are shared out between thread blocks (linear_kernel.cuh).
 //
-// The product is a list of output tiles, each `kb` k-blocks deep (a k-block here is
-// one ring stage of the kernel).  `workers` blocks (or
-// pairs of blocks) run at the same time, one per SM (pair of SMs).  Tiles are dealt out whole, worker c taking tiles
-// c, c + workers, ...; what does not fill a last round -- or everything, where there are fewer tiles than workers, as
-// for a few tokens -- can instead be cut into equal runs of k-blocks, one run per worker.  A run then covers the end of
-// one tile and perhaps the beginning of the next; the pieces of a tile are parked as fp32 in numbered slots of the
-// workspace and added in worker order by whichever of its workers comes last.  Everything is computed from the sizes
-// by every role of every block for itself (group sizes are known on the device only), and the sums do not depend on
-// which worker came last.
+// The product is a list of output tiles, each `kb` k-blocks deep (a k-block here is one ring stage of the kernel).
+// `workers` blocks (or pairs of blocks) run at the same time, one per SM (pair of SMs).  Tiles are dealt out whole, worker c
+// taking tiles c, c + workers, ...; of what does not fill a last round -- or of everything, where there are fewer tiles
+// than workers, as for a few tokens -- every tile can instead be cut into `parts` runs of k-blocks, one run per worker.  The
+// pieces of a tile are parked as fp32 in the workspace, one numbered slot per worker, and added in worker order by whichever of
+// them comes last.  Everything is computed from the sizes by every role of every block for itself (group sizes are known on the
+// device only), and the sums do not depend on which worker came last.
+//
+// Equal parts, although (tiles * parts) workers may be fewer than there are: with runs of equal length over all workers, run
+// borders lie anywhere in a tile, tiles have more pieces and workers two of them (28 tiles of 56 k-blocks on 74 pairs: 37 us,
+// 31 with two parts each on 56 of them).
 #pragma once
 
 #include <cstdint>
@@ -25,51 +27,53 @@ struct LinearPartition {
     int kb;       // k-blocks per tile
     int workers;  // blocks (pairs) of the launch
     int whole;    // tiles 0 .. whole - 1 are dealt out whole
-    int rest;     // tiles whole .. whole + rest - 1 are cut into runs of k-blocks
-    int cutters;  // workers 0 .. cutters - 1 get a run each
+    int rest;     // tiles whole .. whole + rest - 1 are cut
+    int parts;    // into so many runs each
 };
 
 struct LinearSegment {
     int tile;         // < 0: no such segment
     int kb0, kb1;     // its k-blocks
-    int slot;         // where a piece is parked; < 0: the tile is whole
-    int first, last;  // workers that hold the pieces of the tile
+    int first, last;  // workers that hold the pieces of the tile (the same one: the tile is whole)
 };
 
-constexpr int kMaxPieces = 16;  // pieces of one tile: bounds what the last worker has to add up
-constexpr int kMinRun    = 2;   // k-blocks a run has at least
+constexpr int kMinRun = 2;  // k-blocks a run has at least
 
-// overhead: what parking and adding a piece costs, in k-blocks; < 0: no workspace, nothing is cut
-SPMM_B200_HD LinearPartition make_linear_partition(int tiles, int kb, int workers, int overhead)
+// What cutting costs (all in k-blocks of a worker that has the memory system to itself).
+struct LinearCutting {
+    int overhead;    // parking and adding the pieces of a tile; < 0: no workspace, nothing is cut
+    int saturating;  // workers that use all of the memory's bandwidth: more of them take longer over a k-block each
+    int pieces;      // of one tile at most: bounds what the last worker has to add up
+};
+
+SPMM_B200_HD int linear_min(int a, int b)
+{
+    return a < b ? a : b;
+}
+
+SPMM_B200_HD LinearPartition make_linear_partition(int tiles, int kb, int workers, LinearCutting cut)
 {
     LinearPartition p;
     p.kb      = kb;
     p.workers = workers;
     p.rest    = tiles % workers;
     p.whole   = tiles - p.rest;
-    p.cutters = 0;
-    if (p.rest > 0 && overhead >= 0) {
-        const int64_t units   = static_cast<int64_t>(p.rest) * kb;
-        int64_t       cutters = units / kMinRun;
-        if (cutters > static_cast<int64_t>(p.rest) * kMaxPieces)
-            cutters = static_cast<int64_t>(p.rest) * kMaxPieces;
-        if (cutters > workers)
-            cutters = workers;
-        if (cutters > p.rest && (units + cutters - 1) / cutters + overhead < kb)
-            p.cutters = static_cast<int>(cutters);
+    p.parts   = 1;
+    if (p.rest > 0 && cut.overhead >= 0) {
+        const int parts = linear_min(workers / p.rest, linear_min(cut.pieces, kb / kMinRun));
+        if (parts > 1) {
+            const int     run   = (kb - 1) / parts + 1, cutters = p.rest * parts;
+            const int64_t whole = static_cast<int64_t>(kb) * (p.rest > cut.saturating ? p.rest : cut.saturating);
+            const int64_t cost  = static_cast<int64_t>(run) * (cutters > cut.saturating ? cutters : cut.saturating);
+            if (cost + static_cast<int64_t>(cut.overhead) * cut.saturating < whole)
+                p.parts = parts;
+        }
     }
-    if (p.cutters == 0) {
+    if (p.parts == 1) {
         p.whole = tiles;
         p.rest  = 0;
     }
     return p;
-}
-
-// The worker whose run holds k-block `unit` of the `units` that are cut.
-SPMM_B200_HD int linear_cutter_of(const LinearPartition& p, int64_t unit)
-{
-    const int64_t units = static_cast<int64_t>(p.rest) * p.kb;
-    return static_cast<int>(((unit + 1) * p.cutters - 1) / units);
 }
 
 // Segment i (0, 1, ...) of a worker.
@@ -78,36 +82,21 @@ SPMM_B200_HD LinearSegment linear_segment(const LinearPartition& p, int worker, 
     LinearSegment s;
     s.tile = -1;
     s.kb0 = 0, s.kb1 = p.kb;
-    s.slot = -1, s.first = s.last = worker;
+    s.first = s.last = worker;
     const int rounds = worker < p.whole ? (p.whole - worker - 1) / p.workers + 1 : 0;
     if (i < rounds) {
         s.tile = worker + i * p.workers;
         return s;
     }
-    const int part = i - rounds;  // a run covers two tiles at most: there are no fewer cutters than tiles to cut
-    if (worker >= p.cutters || part > 1)
+    if (i > rounds || worker >= p.rest * p.parts)
         return s;
-    const int64_t units = static_cast<int64_t>(p.rest) * p.kb;
-    const int64_t u0 = worker * units / p.cutters, u1 = (worker + 1) * units / p.cutters;
-    const int     t = static_cast<int>(u0 / p.kb) + part;
-    const int64_t begin = static_cast<int64_t>(t) * p.kb, end = begin + p.kb;
-    if (u1 <= begin)
-        return s;
+    const int t = worker / p.parts, part = worker % p.parts;
     s.tile  = p.whole + t;
-    s.kb0   = part == 0 ? static_cast<int>(u0 - begin) : 0;
-    s.kb1   = static_cast<int>((u1 < end ? u1 : end) - begin);
-    s.first = linear_cutter_of(p, begin);
-    s.last  = linear_cutter_of(p, end - 1);
-    if (s.first != s.last)
-        s.slot = 2 * worker + part;
+    s.kb0   = static_cast<int>(static_cast<int64_t>(p.kb) * part / p.parts);
+    s.kb1   = static_cast<int>(static_cast<int64_t>(p.kb) * (part + 1) / p.parts);
+    s.first = t * p.parts;
+    s.last  = s.first + p.parts - 1;
     return s;
-}
-
-// The slot in which worker `w` parks its piece of the tile that segment `s` belongs to.
-SPMM_B200_HD int linear_slot_of(const LinearPartition& p, const LinearSegment& s, int w)
-{
-    const int64_t units = static_cast<int64_t>(p.rest) * p.kb;
-    return 2 * w + (w * units / p.cutters < static_cast<int64_t>(s.tile - p.whole) * p.kb ? 1 : 0);
 }
 
 }  // namespace spmm_b200

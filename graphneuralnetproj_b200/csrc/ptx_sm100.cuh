@@ -235,6 +235,22 @@ tma_load_3d_pair(uint32_t dst_smem, const void* tensor_map, int x, int y, int z,
         : "memory");
 }
 
+// Asks for a tensor map itself, ahead of the first load that uses it.
+__device__ __forceinline__ void prefetch_tensor_map(const void* tensor_map)
+{
+    asm volatile("prefetch.tensormap [%0];" ::"l"(tensor_map) : "memory");
+}
+
+// Barrier `id` of the block among `threads` threads: arriving without waiting, and waiting.
+__device__ __forceinline__ void named_arrive(int id, int threads)
+{
+    asm volatile("barrier.cta.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void named_sync(int id, int threads)
+{
+    asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
 // Asks the memory system to bring `bytes` (a multiple of 16, from a 16-byte aligned address) into L2.
 __device__ __forceinline__ void bulk_prefetch_l2(const void* src, uint32_t bytes)
 {

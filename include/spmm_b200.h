@@ -401,10 +401,11 @@ int spmm_b200_grouped_fp8_linear(void*        stream,
                                  void*        workspace,
                                  size_t       workspace_bytes);
 
-/* Segment `index` of the share of tiles that block `worker` of a linear layer gets (for tests of the host logic):
- * segment[7] = tile (-1: no such segment), first and past-the-last k-block, workspace slot or -1, first and last
- * worker with a piece of the tile, and the slot the adding worker reads this piece from. */
-int spmm_b200_linear_plan(int tiles, int kb, int workers, int overhead, int worker, int index, int* segment);
+/* Segment `index` of the share of tiles that block `worker` of a linear layer gets (for tests of the host logic;
+ * overhead, saturating, pieces: LinearCutting in csrc/linear_plan.h):
+ * segment[5] = tile (-1: no such segment), first and past-the-last k-block, first and last worker with a piece of the tile. */
+int spmm_b200_linear_plan(
+    int tiles, int kb, int workers, int overhead, int saturating, int pieces, int worker, int index, int* segment);
 
 /* Device-side status of the current device: 0 = ok, 1 = a bounded wait inside a
  * kernel gave up.  Synchronises the device.  With reset != 0 the status and the

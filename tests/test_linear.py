@@ -11,34 +11,39 @@ def test_plan_covers_every_k_block_once(sp, workers, overhead):
     rng = random.Random(workers * 100 + overhead)
     for tiles, kb in [(0, 5), (1, 1), (1, 300), (workers, 7), (workers + 1, 64), (2 * workers - 1, 3)] + \
             [(rng.randint(1, 500), rng.randint(1, 300)) for _ in range(30)]:
-        pieces, slots = {}, set()
+        pieces = {}
         for worker, segments in enumerate(sp.linear_plan(tiles, kb, workers, overhead)):
-            for tile, k0, k1, slot, first, last, read_from in segments:
+            # a worker parks at most one piece: it has one slot
+            assert sum(first != last for _, _, _, first, last in segments) <= 1
+            for tile, k0, k1, first, last in segments:
                 assert 0 <= tile < tiles and 0 <= k0 < k1 <= kb
-                pieces.setdefault(tile, []).append((k0, k1, worker, slot, first, last))
-                if slot >= 0:  # parked where the adding worker looks for it, and nobody else parks there
-                    assert slot == read_from and slot < 2 * workers and slot not in slots
-                    slots.add(slot)
+                pieces.setdefault(tile, []).append((k0, k1, worker, first, last))
         assert sorted(pieces) == list(range(tiles))
         counters = set()
         for parts in pieces.values():
             parts.sort()
             assert parts[0][0] == 0 and parts[-1][1] == kb and all(a[1] == b[0] for a, b in zip(parts, parts[1:]))
-            assert (len(parts) == 1) == (parts[0][3] < 0)
             owners = [p[2] for p in parts]
-            assert owners == list(range(owners[0], owners[-1] + 1)) and len(owners) <= 17
-            assert all(p[4] == owners[0] and p[5] == owners[-1] for p in parts)
+            assert owners == list(range(owners[0], owners[-1] + 1)) and len(owners) <= 16
+            assert all(p[3] == owners[0] and p[4] == owners[-1] for p in parts)
+            assert overhead >= 0 or len(parts) == 1
             if len(parts) > 1:  # arrivals are counted under the first owner
                 assert owners[0] not in counters
                 counters.add(owners[0])
-        if overhead < 0:
-            assert not slots
 
 
 def test_plan_evens_out_few_tiles(sp):
-    """72 tiles of 72 k-blocks on 148 workers: nobody has more than its share, rounded up."""
+    """72 tiles of 72 k-blocks on 148 workers: two equal parts each."""
     plan = sp.linear_plan(72, 72, 148, 4)
-    assert max(sum(s[2] - s[1] for s in segments) for segments in plan) == -(-72 * 72 // 148)
+    assert sorted(sum(s[2] - s[1] for s in segments) for segments in plan) == [0] * 4 + [36] * 144
+
+
+def test_plan_cuts_only_where_it_pays(sp):
+    whole = [(0, 0, 16, 0, 0)]
+    assert sp.linear_plan(1, 16, 148, 17, 91)[0] == whole  # 2 k-blocks and 17 of overhead are more than 16
+    assert len([w for w in sp.linear_plan(1, 36, 148, 17, 91) if w]) == 16
+    assert all(len(w) == 1 for w in sp.linear_plan(72, 36, 148, 17, 91)[:72])  # 144 workers would share the bandwidth of 91
+    assert sp.linear_plan(75, 56, 148, 0)[74] == [(74, 0, 56, 74, 74)]  # not two workers for every tile
 
 
 def test_workspace_bytes(sp):
