@@ -74,10 +74,16 @@ __device__ __forceinline__ float scale_of(uint32_t amax16)
     return fmaxf(__fdiv_rn(element<BF16>(amax16), kE4m3Max), kScaleMin);
 }
 
-__device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi)
+// Four codes, the first in the lowest byte.
+__device__ __forceinline__ uint32_t e4m3_quad(float x0, float x1, float x2, float x3)
 {
-    uint16_t out;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(out) : "f"(hi), "f"(lo));
+    uint32_t out;
+    asm("{\n\t.reg .b16 lo, hi;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+        "mov.b32 %0, {lo, hi};\n\t}"
+        : "=r"(out)
+        : "f"(x0), "f"(x1), "f"(x2), "f"(x3));
     return out;
 }
 
@@ -117,19 +123,26 @@ __device__ __forceinline__ uint2 encode8(uint4 v, BlockScale s, bool redo)
         for (int i = 0; i < 4; i++)
             w[i] |= __vcmpgeu2(w[i] & 0x7fff7fffu, kInfPair<BF16>);
     }
-    uint32_t lo[4], hi[4];
+    float x[8];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const float x0 = element<BF16>(w[i] & 0xffffu), x1 = element<BF16>(w[i] >> 16);
-        lo[i] = e4m3_pair(x0 * s.below, x1 * s.below);
-        hi[i] = e4m3_pair(x0 * s.above, x1 * s.above);
+        x[2 * i]     = element<BF16>(w[i] & 0xffffu);
+        x[2 * i + 1] = element<BF16>(w[i] >> 16);
     }
-    if ((lo[0] | (lo[1] << 16)) != (hi[0] | (hi[1] << 16)) || (lo[2] | (lo[3] << 16)) != (hi[2] | (hi[3] << 16))) {
+    uint32_t lo[2], hi[2];
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            lo[i] = settle(lo[i], hi[i], element<BF16>(w[i] & 0xffffu), element<BF16>(w[i] >> 16), s.scale);
+    for (int i = 0; i < 2; i++) {
+        const float* y = x + 4 * i;
+        lo[i] = e4m3_quad(y[0] * s.below, y[1] * s.below, y[2] * s.below, y[3] * s.below);
+        hi[i] = e4m3_quad(y[0] * s.above, y[1] * s.above, y[2] * s.above, y[3] * s.above);
     }
-    return make_uint2(lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16));
+    if (lo[0] != hi[0] || lo[1] != hi[1]) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            lo[i] = settle(lo[i] & 0xffffu, hi[i] & 0xffffu, x[4 * i], x[4 * i + 1], s.scale)
+                    | (settle(lo[i] >> 16, hi[i] >> 16, x[4 * i + 2], x[4 * i + 3], s.scale) << 16);
+    }
+    return make_uint2(lo[0], lo[1]);
 }
 
 template<bool BF16>
