@@ -141,7 +141,7 @@ cudaError_t launch(cudaStream_t stream, LinearParams& p, const LinearShape& s)
     p.steps               = PAIR ? s.kb : (s.kb - 1) / kStepBlocks + 1;
 
     cudaLaunchConfig_t config = {};
-    config.blockDim           = dim3(PAIR ? kPairThreads<EIGHT> : kLinearThreads);
+    config.blockDim           = dim3(kLinearThreads);
     config.dynamicSmemBytes   = fixed + p.stages * stage_bytes;
     config.stream             = stream;
     cudaLaunchAttribute attr[2];

@@ -17,6 +17,13 @@
 // in every step, the few hundred instructions of the epilogue warps around them took 1.4 us per step, twice what the
 // 32 KB of a step take to arrive (36864 x 9216, 16 tokens: 104 us, against 70 without the second wait).
 //
+// What bounds it: memory.  A block has six stages of 36 KB on their way at 16 tokens; 36864 x 9216 in 8 bits and 16 tokens take
+// 57 us (341 MB, 0.91 of the measured copy bandwidth), 64 experts of 2048 x 4096 in bf16 and 96 tokens 114 us (0.97).  A launch
+// has about 5 us that do not depend on the size (first loads, last tile's way out), which is what a small layer costs.
+//
+// MMAs, commits and TMA loads are issued by an elected lane in code that is uniform for the compiler (values that come out of
+// shared memory pass through linear_uniform): under `lane == 0` four MMAs and two commits took 520 cycles, now 170.
+//
 // Roles: warp 0 TMA, warp 1 MMA issue and TMEM, warp 2 scales, warps 4..11 epilogue (warp % 4 = quarter of the TMEM
 // lanes, warp / 4 - 1 = every other chunk of columns).  Every wait is bounded; a block that gives up records it.
 #pragma once
@@ -115,7 +122,7 @@ __device__ __forceinline__ int linear_tile_rows(int rows, int tile_tokens, int g
 // Fills the table; all threads of the block, with block barriers.  Borders are clamped to the tokens there are, so that a
 // corrupt table cannot lead outside.  Tiles are up to `tile_tokens` tokens x one of `tiles_m` blocks of rows of A.
 // sort: groups with wider tiles first.  Whole tiles are dealt to the blocks in turn, so that blocks get tiles of about the same
-// width only if neighbours in the list have it (16 groups of 124 to 2220 tokens: 565 -> 460 us with equal tiles and sorting).
+// width only if neighbours in the list have it (16 groups of 124 to 2220 tokens: 542 -> 476 us with equal tiles and sorting).
 template<bool SORT>
 __device__ __forceinline__ void
 linear_build_table(const LinearParams& p, const LinearTable& table, int* warp_sums, int tile_tokens, int granule, int tiles_m)

@@ -10,12 +10,21 @@
 // Codes: tokens on the lanes, weights as columns.  Every k-block is a product of its own that the epilogue warps add to
 // fp32 registers (128 of them per thread: two warpgroups share the 256 columns) while the tensor core fills the other
 // half of TMEM.  This way round a thread's factor is one number per k-block, (its token's scale) * (the scale of its 128
-// columns), and the addition two columns per instruction; with tokens as columns each column needs its own factor out of
-// shared memory, which costs as much of shared memory's time as the operands do.
+// columns); with tokens as columns each column needs its own factor out of shared memory, which costs as much of shared
+// memory's time as the operands do.
 //
-// Roles per block as in the single-block kernel without the scale warp; the even block's (the leader's) warp 1 issues the
-// pair's MMAs.  The "full" and "acc_free" barriers live in the leader; commits arrive in both blocks.  Every wait is
-// bounded, and both blocks meet at a cluster barrier before they exit.
+// What bounds them.  16 bits: the tensor core (2048 x 9472 x 4096: 112 us against 97 at the measured cuBLAS rate, tensor pipe
+// active 78 %).  Codes: the additions beside the MMAs.  A k-block takes 1000 cycles (2048 x 9472 x 8192: 154 us, tensor pipe
+// 48 %), 690 with the additions left out, which alone take 400: 128 per thread and k-block, i.e. 256 issue slots of each
+// scheduler for 512 cycles of MMA, between two hand-overs that each cost a few hundred cycles (commit to wake-up, arrival at the
+// leader to the next MMA).  Measured and dropped: four warpgroups (9 % slower, bound by issue), 256 x 128 tiles with four TMEM
+// buffers (8 % slower), two columns per instruction (fma.rn.f32x2 runs at half rate and costs register moves), spinning
+// instead of parked waits (no change), half as many instructions around the additions (no change).
+//
+// Roles per block as in the single-block kernel, with warps 2 and 3 for the scales; the even block's (the leader's) warp 1
+// issues the pair's MMAs, a commit arrives in both blocks.  The "full" and "acc_free" barriers live in the leader; arrivals
+// there need no cluster-scope release (mbar_arrive_remote), which took over 1000 cycles each.  Every wait is bounded, and both
+// blocks meet at a cluster barrier before they exit.
 #pragma once
 
 #include "linear_kernel.cuh"
@@ -27,20 +36,13 @@ constexpr int kPairStageBytes = 2 * kLinearBoxBytes;
 constexpr int kPairStages     = 7;  // at most
 constexpr int kPairBatch      = 8;  // k-blocks whose factors are handed over together
 
-// Epilogue warps: two warpgroups read 16-bit products out of TMEM once per tile; four share the additions of every k-block.
 template<bool EIGHT>
-constexpr int kPairEpilogueWarps = 8;
-template<bool EIGHT>
-constexpr int kPairThreads = 128 + 32 * kPairEpilogueWarps<EIGHT>;
-
-template<bool EIGHT>
-__global__ void __launch_bounds__(kPairThreads<EIGHT>, 1)
+__global__ void __launch_bounds__(kLinearThreads, 1)
 linear_pair_kernel(const __grid_constant__ LinearParams p)
 {
-    constexpr int EPI   = kPairEpilogueWarps<EIGHT>;
-    constexpr int TEAMS = EPI / 4;                   // warps per quarter of the lanes
-    constexpr int CH    = EIGHT ? 32 : 16;           // columns per chunk
-    constexpr int NCH   = kPairTile / (TEAMS * CH);  // chunks per epilogue warp
+    constexpr int EPI = kEpilogueTeams;           // epilogue warps
+    constexpr int CH  = EIGHT ? 32 : 16;          // columns per chunk
+    constexpr int NCH = kPairTile / (2 * CH);     // chunks per epilogue warp
 
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (ptx::smem_addr(smem_raw) + 1023u) & ~1023u;
@@ -261,7 +263,7 @@ linear_pair_kernel(const __grid_constant__ LinearParams p)
         const int      row     = (warp & 3) * 32 + lane;
         const uint32_t tmem_at = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t leader_acc_free0 = ptx::map_to_cta(acc_free(0), 0);
-        auto           col_of  = [&](int c) { return EIGHT ? (team * NCH + c) * CH : (TEAMS * c + team) * CH; };
+        auto           col_of  = [&](int c) { return EIGHT ? (team * NCH + c) * CH : (2 * c + team) * CH; };
         uint32_t       use     = 0, batch = 0;
         bool           ok      = true;
         for (int i = 0; ok; i++) {

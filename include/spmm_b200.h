@@ -349,7 +349,8 @@ int spmm_b200_quantize_fp8(
  * (few tokens, or a last round of tiles that does not fill the GPU); 0 for sizes they refuse.  With less, or
  * none, they run without cutting, at the same results within the rounding of the sums.  A workspace is filled
  * with zeros once, before its first use; every call leaves it ready for the next, of any size it is large enough
- * for.  Calls that may run at the same time need different workspaces (also calls captured in graphs that may). */
+ * for.  Calls that may run at the same time need different workspaces (also calls captured in graphs that may).
+ * After spmm_b200_device_status has reported that a wait gave up, fill it with zeros again. */
 size_t spmm_b200_linear_workspace_bytes(int groups, int M_Global, int N_Global, int K_Global, int eight_bit);
 
 /* C = B * A^T from codes and scales.  K a multiple of 16; any M and N.  C_type: type of C. */
