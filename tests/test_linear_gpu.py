@@ -247,6 +247,76 @@ def test_two_streams_at_once_and_graph_replay(sp):
             check(c, av, bv, borders(table), k, torch.float16)
 
 
+@pytest.mark.parametrize("kind", ["e4m3", "bf16"])
+def test_pairs_on_two_streams_and_in_a_graph(sp, kind):
+    """Many tokens per group: two calls at once with a workspace each, then both in one graph, K cut between pairs."""
+    m, k, sizes = 512, 8192, [200, 0, 310]
+    n, dtype = sum(sizes), None if kind == "e4m3" else torch.bfloat16
+    off = torch.tensor(borders(sizes), dtype=torch.int32, device="cuda")
+    jobs = []
+    for seed in (1, 2):
+        a, sa, b, sb, av, bv = random_operands(3, m, n, k, dtype, seed)
+        jobs.append((a, sa, b, sb, torch.full((n, m), 7.0, dtype=torch.bfloat16, device="cuda"), workspace_for(sp, 3, m, n, k, dtype is None), av, bv))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        for s, (a, sa, b, sb, c, ws, _, _) in zip(streams, jobs):
+            assert call(sp, a, sa, b, sb, c, off, 3, m, n, k, ws, s.cuda_stream) == 0  # a raw handle
+    torch.cuda.synchronize()
+    first = [job[4].clone() for job in jobs]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for a, sa, b, sb, c, ws, _, _ in jobs:
+            assert call(sp, a, sa, b, sb, c, off, 3, m, n, k, ws) == 0
+    for job in jobs:
+        job[4].fill_(7.0)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert sp.device_status() == 0
+    for (_, _, _, _, c, _, av, bv), before in zip(jobs, first):
+        assert torch.equal(c, before)
+        check(c, av, bv, borders(sizes), k, torch.bfloat16)
+
+
+def test_smallest_depth_and_codes_as_bytes(sp):
+    """K of one 16-byte row; codes passed as uint8."""
+    run_case(sp, 2, 3, 5, 8, torch.float16, torch.float16, [0, 2, 5], True, integer_operands, True)
+    m, n, k = 72, 9, 16
+    a, sa, b, sb, av, bv = integer_operands(1, m, n, k, None, 2)
+    c = torch.full((n, m), 7.0, dtype=torch.bfloat16, device="cuda")
+    assert sp.fp8_linear(None, a.view(torch.uint8), sa, b.view(torch.uint8), sb, c, m, n, k, None) == 0
+    assert torch.equal(c.double(), bv @ av[0].t())
+
+
+def test_nothing_to_do(sp):
+    """No tokens, no rows: nothing is written."""
+    m, k = 128, 128
+    a, sa, _, _, _, _ = random_operands(2, m, 1, k, None, 3)
+    empty8, empty = torch.empty((0, k), dtype=torch.float8_e4m3fn, device="cuda"), torch.empty((0, m), dtype=torch.float16, device="cuda")
+    scales, off = torch.empty((1, 0), device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    assert sp.fp8_linear(None, a[0], sa[0], empty8, scales, empty, m, 0, k, None) == 0
+    assert sp.grouped_fp8_linear(None, a, sa, empty8, scales, empty, off, 2, m, 0, k, None) == 0
+    assert sp.grouped_linear(None, a.to(torch.float16), empty8.to(torch.float16), empty, off, 2, m, 0, k, None) == 0
+    assert sp.quantize_fp8(None, torch.empty((0, k), dtype=torch.float16, device="cuda"), empty8, scales, 1) == 0
+
+
+def test_not_finite_operands_reach_their_rows_only(sp):
+    """Infinite activations or scales spoil the tokens they belong to, at few and at many tokens."""
+    for n in (20, 300):
+        m, k = 136, 400
+        a, sa, b, sb, av, bv = random_operands(1, m, n, k, None, 8)
+        sb = sb.clone()
+        sb[1, 7] = float("inf")
+        sb[3, 11] = float("nan")
+        c = torch.full((n, m), 7.0, dtype=torch.bfloat16, device="cuda")
+        assert sp.fp8_linear(None, a[0], sa[0], b, sb, c, m, n, k, workspace_for(sp, 1, m, n, k, True)) == 0
+        assert not bool(c[[7, 11]].isfinite().any())
+        good = torch.ones(n, dtype=torch.bool, device="cuda")
+        good[[7, 11]] = False
+        check(c[good], av, bv[good], None, k, torch.bfloat16)
+
+
 # ---------------------------------------------------------------- quantiser
 def reference_codes(x, block_rows):
     """(values, scales) by the definition: the e4m3 value nearest to x / scale, ties to the even code."""
