@@ -14,12 +14,14 @@
 // memory's time as the operands do.
 //
 // What bounds them.  16 bits: the tensor core (2048 x 9472 x 4096: 112 us against 97 at the measured cuBLAS rate, tensor pipe
-// active 78 %).  Codes: the additions beside the MMAs.  A k-block takes 1000 cycles (2048 x 9472 x 8192: 154 us, tensor pipe
-// 48 %), 690 with the additions left out, which alone take 400: 128 per thread and k-block, i.e. 256 issue slots of each
-// scheduler for 512 cycles of MMA, between two hand-overs that each cost a few hundred cycles (commit to wake-up, arrival at the
-// leader to the next MMA).  Measured and dropped: four warpgroups (9 % slower, bound by issue), 256 x 128 tiles with four TMEM
-// buffers (8 % slower), two columns per instruction (fma.rn.f32x2 runs at half rate and costs register moves), spinning
-// instead of parked waits (no change), half as many instructions around the additions (no change).
+// active 78 %).  Codes: the way round a TMEM buffer -- MMA, commit, wake-up, read-out, additions, arrival at the leader, next MMA --
+// of which there are two.  A k-block takes 0.51 us, about 840 cycles (2048 x 9472 x 8192: 148 us, tensor pipe 48 %); 0.46 without
+// the TMA loads, 0.48 without the scales, 0.40 without both; the protocol by itself, on operands that stay in shared memory, takes
+// 600 cycles, without the additions the 512 of the MMA.  (Additions that never stall starve the MMA warp of their scheduler: 909
+// cycles; the reads out of TMEM between them prevent that.)  Measured and dropped: four warpgroups (9 % slower, bound by
+// issue), 256 x 128 tiles with four buffers (8 % slower), a k-block as two products of 128 columns in four buffers (2 %
+// slower), two columns per instruction (fma.rn.f32x2 runs at half rate and costs register moves), spinning instead of parked
+// waits, half as many instructions around the additions (no change).
 //
 // Roles per block as in the single-block kernel, with warps 2 and 3 for the scales; the even block's (the leader's) warp 1
 // issues the pair's MMAs, a commit arrives in both blocks.  The "full" and "acc_free" barriers live in the leader; arrivals
