@@ -390,13 +390,7 @@ linear_pair_kernel(const __grid_constant__ LinearParams p)
                     }
                     return;
                 }
-                const int m = t.m0 + static_cast<int>(rank) * kLinearRows + row;
-                if (m >= p.m)
-                    return;
-#pragma unroll
-                for (int j = 0; j < CH; j++)
-                    if (col_of(c) + j < t.rows)
-                        linear_store(p, static_cast<size_t>(t.row0 + col_of(c) + j) * p.m + m, v[j]);
+                linear_store_columns<CH>(p, t, t.m0 + static_cast<int>(rank) * kLinearRows + row, col_of(c), v);
             };
             if (seg.first == seg.last) {
 #pragma unroll
