@@ -64,19 +64,17 @@ int max_workers(const LinearShape& s)
     return s.pair ? kMaxWorkers / 2 : kMaxWorkers;
 }
 
-// When cutting tiles pays (linear_plan.h), from measurements.  Few tokens: a block streams a step (32 KB) in 0.43 us while at
-// most about 90 do; cutting costs 4 us up to 32 tokens (1 token, 4096 x 4096, 32 tiles of 16 steps: 11.5 us whole, 10.2 in four
-// parts; 9216 x 9216, 72 of 36: 20.7 and 25), 7 us up to 64 (64 x 2048 x 4096: 13.9 and 15.5).  Over 64 tokens a step takes as
-// long as its arithmetic, about 1 us (90 x 4096 x 2048, 32 tiles of 8: 12.1 and 15.3; 100 x 7168 x 7168, 56 of 28: 38 and 24.6).
-// Pairs: a piece is 128 KB per block, a k-block 0.57 us (512 x 4096 x 14336, 32 tiles of 112: 60 us whole, 43 in two parts; 200 x
-// 2048 x 2048, 8 of 16: 14.8 and 19.1).
+// When cutting tiles pays (linear_plan.h), from measurements.  Few tokens: a block streams a step (32 KB) in 0.43 us, cutting costs
+// 4 us up to 32 tokens (1 token, 4096 x 4096, 32 tiles of 16 steps: 11.5 us whole, 10.6 in three parts; 9216 x 9216, 72 of 36: 20.7
+// and 21.4 where memory answers fast, 39 and 30 where it does not, and twice the blocks have twice the loads on their way), 7 us
+// up to 64 (64 x 2048 x 4096: 13.9 and 15.5).  Over 64 tokens a step takes as long as its arithmetic, about 1 us (90 x 4096 x
+// 2048, 32 tiles of 8: 12.1 and 15.3; 100 x 7168 x 7168, 56 of 28: 38 and 24.6).  Pairs: a piece is 128 KB per block, a k-block
+// 0.5 us (512 x 4096 x 14336, 32 tiles of 112: 60 us whole, 43 in two parts; 200 x 2048 x 2048, 8 of 16: 14.8 and 19.1).
 LinearCutting cutting(const LinearShape& s)
 {
     if (s.pair)
-        return LinearCutting{14, max_workers(s), 4};
-    if (s.nt <= 64)
-        return LinearCutting{s.nt <= 32 ? 9 : 17, 91, 16};
-    return LinearCutting{8, max_workers(s), 16};
+        return LinearCutting{14, 4};
+    return LinearCutting{s.nt <= 32 ? 9 : (s.nt <= 64 ? 17 : 8), 16};
 }
 
 size_t workspace_needed(const LinearShape& s)
@@ -342,12 +340,12 @@ int spmm_b200_grouped_fp8_linear(void*        stream,
                                    B, B_scales, C, C_type, group_offsets, workspace, workspace_bytes));
 }
 
-int spmm_b200_linear_plan(int tiles, int kb, int workers, int overhead, int saturating, int pieces, int worker, int index, int* segment)
+int spmm_b200_linear_plan(int tiles, int kb, int workers, int overhead, int pieces, int worker, int index, int* segment)
 {
     using namespace spmm_b200;
-    if (tiles < 0 || kb < 1 || workers < 1 || saturating < 1 || pieces < 1 || worker < 0 || worker >= workers || index < 0 || !segment)
+    if (tiles < 0 || kb < 1 || workers < 1 || pieces < 1 || worker < 0 || worker >= workers || index < 0 || !segment)
         return static_cast<int>(cudaErrorInvalidValue);
-    const LinearPartition p = make_linear_partition(tiles, kb, workers, LinearCutting{overhead, saturating, pieces});
+    const LinearPartition p = make_linear_partition(tiles, kb, workers, LinearCutting{overhead, pieces});
     const LinearSegment   s = linear_segment(p, worker, index);
     segment[0] = s.tile;
     segment[1] = s.kb0;

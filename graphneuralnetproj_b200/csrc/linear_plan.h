@@ -39,11 +39,9 @@ struct LinearSegment {
 
 constexpr int kMinRun = 2;  // k-blocks a run has at least
 
-// What cutting costs (all in k-blocks of a worker that has the memory system to itself).
 struct LinearCutting {
-    int overhead;    // parking and adding the pieces of a tile; < 0: no workspace, nothing is cut
-    int saturating;  // workers that use all of the memory's bandwidth: more of them take longer over a k-block each
-    int pieces;      // of one tile at most: bounds what the last worker has to add up
+    int overhead;  // what parking and adding the pieces of a tile costs, in k-blocks; < 0: no workspace, nothing is cut
+    int pieces;    // of one tile at most: bounds what the last worker has to add up
 };
 
 SPMM_B200_HD int linear_min(int a, int b)
@@ -65,13 +63,8 @@ SPMM_B200_HD LinearPartition make_linear_partition(int tiles, int kb, int worker
         int parts = linear_min(workers / p.rest, linear_min(cut.pieces, kb / kMinRun));
         while (parts > 1 && 7 * parts * parts > 5 * kb)
             parts--;
-        if (parts > 1) {
-            const int     run   = (kb - 1) / parts + 1, cutters = p.rest * parts;
-            const int64_t whole = static_cast<int64_t>(kb) * (p.rest > cut.saturating ? p.rest : cut.saturating);
-            const int64_t cost  = static_cast<int64_t>(run) * (cutters > cut.saturating ? cutters : cut.saturating);
-            if (cost + static_cast<int64_t>(cut.overhead) * cut.saturating < whole)
-                p.parts = parts;
-        }
+        if (parts > 1 && (kb - 1) / parts + 1 + cut.overhead < kb)
+            p.parts = parts;
     }
     if (p.parts == 1) {
         p.whole = tiles;

@@ -125,7 +125,7 @@ def _load():
     lib.spmm_b200_grouped_linear.restype = ci
     lib.spmm_b200_grouped_fp8_linear.argtypes = [vp] * 6 + [ci, vp] + [ci] * 4 + [vp, sz]
     lib.spmm_b200_grouped_fp8_linear.restype = ci
-    lib.spmm_b200_linear_plan.argtypes = [ci] * 8 + [_i32p]
+    lib.spmm_b200_linear_plan.argtypes = [ci] * 7 + [_i32p]
     lib.spmm_b200_linear_plan.restype = ci
     lib.spmm_b200_plan.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_long, _i32p, _i32p, _i32p]
     lib.spmm_b200_plan.restype = ctypes.c_int
@@ -394,14 +394,14 @@ def grouped_fp8_linear(stream, A, A_scales, B, B_scales, C, group_offsets, group
                                             ws, ws_bytes)
 
 
-def linear_plan(tiles, kb, workers, overhead, saturating=None, pieces=16):
+def linear_plan(tiles, kb, workers, overhead, pieces=16):
     """How the linear layers share out `tiles` tiles of `kb` k-blocks: per worker a list of (tile, first k-block, past the
     last, first and last worker with a piece of the tile)."""
     plan, segment = [], (ctypes.c_int * 5)()
     for worker in range(workers):
         plan.append([])
         while True:
-            if LIB.spmm_b200_linear_plan(tiles, kb, workers, overhead, saturating or workers, pieces, worker, len(plan[-1]), segment) != 0:
+            if LIB.spmm_b200_linear_plan(tiles, kb, workers, overhead, pieces, worker, len(plan[-1]), segment) != 0:
                 raise ValueError("no such plan")
             if segment[0] < 0:
                 break

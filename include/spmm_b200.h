@@ -403,10 +403,9 @@ int spmm_b200_grouped_fp8_linear(void*        stream,
                                  size_t       workspace_bytes);
 
 /* Segment `index` of the share of tiles that block `worker` of a linear layer gets (for tests of the host logic;
- * overhead, saturating, pieces: LinearCutting in csrc/linear_plan.h):
+ * overhead, pieces: LinearCutting in csrc/linear_plan.h):
  * segment[5] = tile (-1: no such segment), first and past-the-last k-block, first and last worker with a piece of the tile. */
-int spmm_b200_linear_plan(
-    int tiles, int kb, int workers, int overhead, int saturating, int pieces, int worker, int index, int* segment);
+int spmm_b200_linear_plan(int tiles, int kb, int workers, int overhead, int pieces, int worker, int index, int* segment);
 
 /* Device-side status of the current device: 0 = ok, 1 = a bounded wait inside a
  * kernel gave up.  Synchronises the device.  With reset != 0 the status and the

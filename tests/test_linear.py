@@ -40,10 +40,10 @@ def test_plan_evens_out_few_tiles(sp):
 
 def test_plan_cuts_only_where_it_pays(sp):
     whole = [(0, 0, 16, 0, 0)]
-    assert sp.linear_plan(1, 16, 148, 17, 91)[0] == whole  # 2 k-blocks and 17 of overhead are more than 16
-    assert len([w for w in sp.linear_plan(1, 36, 148, 17, 91) if w]) == 5  # 7 * 5 * 5 <= 5 * 36
-    assert len([w for w in sp.linear_plan(1, 1000, 148, 17, 91) if w]) == 16
-    assert all(len(w) == 1 for w in sp.linear_plan(72, 36, 148, 17, 91)[:72])  # 144 workers would share the bandwidth of 91
+    assert sp.linear_plan(1, 16, 148, 17)[0] == whole  # 6 k-blocks and 17 of overhead are more than 16
+    assert len([w for w in sp.linear_plan(1, 36, 148, 17) if w]) == 5  # 7 * 5 * 5 <= 5 * 36
+    assert len([w for w in sp.linear_plan(1, 1000, 148, 17) if w]) == 16
+    assert len([w for w in sp.linear_plan(1, 1000, 148, 17, 4) if w]) == 4
     assert sp.linear_plan(75, 56, 148, 0)[74] == [(74, 0, 56, 74, 74)]  # not two workers for every tile
 
 
