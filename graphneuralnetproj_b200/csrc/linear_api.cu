@@ -82,12 +82,17 @@ size_t workspace_needed(const LinearShape& s)
     return kCounterBytes + static_cast<size_t>(max_workers(s)) * s.slot_bytes;
 }
 
-// Sizes that the format and the index arithmetic can describe.
+// Sizes that the format and the index arithmetic can describe.  Tokens: the columns of the last tile behind the last token
+// have numbers too, which have to fit an int.  Depth: the byte offset in a row has to; with 16 bits the whole depth of a tile is
+// one accumulation (half a microsecond per 64) that the epilogue waits for, and a wait gives up after two seconds.
+constexpr int kMaxTokens  = 0x7fffffff - 2 * kPairTile;
+constexpr int kMaxDepth8  = 1 << 29;
+constexpr int kMaxDepth16 = 1 << 27;
+
 bool valid_shape(const LinearShape& s)
 {
-    if (s.m < 1 || s.n < 0 || s.k < 1 || s.groups < 1 || s.groups > kLinearMaxGroups || s.k > (1 << 29) || s.k % (s.eight ? 16 : 8) != 0)
-        return false;
-    return true;
+    return s.m >= 1 && s.n >= 0 && s.n <= kMaxTokens && s.k >= 1 && s.k <= (s.eight ? kMaxDepth8 : kMaxDepth16) && s.k % (s.eight ? 16 : 8) == 0
+           && s.groups >= 1 && s.groups <= kLinearMaxGroups;
 }
 
 cudaError_t describe(CUtensorMap& map, const void* base, long row_bytes, long rows, long groups, int box_rows)

@@ -142,11 +142,17 @@ struct LinearTable {
 constexpr int kLinearTableWords = 4;  // per group
 constexpr int kLinearSortGroups = 256;
 
+// Parts of `by` that cover `count`: not negative, and up to INT_MAX, where a sum of the two no longer fits an int.
+__device__ __forceinline__ int linear_cover(int count, int by)
+{
+    return static_cast<int>((static_cast<unsigned>(count) + static_cast<unsigned>(by) - 1u) / static_cast<unsigned>(by));
+}
+
 // Tokens per tile of a group: the tiles of a group are as wide as one another, in steps of `granule` columns.
 __device__ __forceinline__ int linear_tile_rows(int rows, int tile_tokens, int granule)
 {
-    const int tiles = (rows + tile_tokens - 1) / tile_tokens;
-    return tiles == 0 ? 0 : ((rows + tiles - 1) / tiles + granule - 1) / granule * granule;
+    const int tiles = linear_cover(rows, tile_tokens);
+    return tiles == 0 ? 0 : linear_cover(linear_cover(rows, tiles), granule) * granule;
 }
 
 // Fills the table; all threads of the block, with block barriers.  Borders are clamped to the tokens there are, so that a
@@ -192,7 +198,7 @@ linear_build_table(const LinearParams& p, const LinearTable& table, int* warp_su
     }
     int sum = 0;
     for (int e = e0; e < e1; e++) {
-        sum += (table.rows[e] + tile_tokens - 1) / tile_tokens * tiles_m;
+        sum += linear_cover(table.rows[e], tile_tokens) * tiles_m;
         table.end[e] = sum;
     }
     int before = sum;  // becomes the total of the threads before this one
@@ -227,7 +233,7 @@ linear_locate(const LinearParams& p, const LinearTable& table, int tile, int til
             lo = mid + 1;
     }
     LinearTile t;
-    const int  rows = table.rows[lo], tiles_n = (rows + tile_tokens - 1) / tile_tokens;
+    const int  rows = table.rows[lo], tiles_n = linear_cover(rows, tile_tokens);
     const int  width = linear_tile_rows(rows, tile_tokens, granule);
     const int  i    = tile - (lo > 0 ? table.end[lo - 1] : 0);
     const int  band = i / (kLinearBand * tiles_m), wide = min(kLinearBand, tiles_n - band * kLinearBand);
@@ -358,7 +364,7 @@ linear_kernel(const __grid_constant__ LinearParams p)
             table.row[0]   = 0;
             table.rows[0]  = p.n;
             table.group[0] = 0;
-            table.end[0]   = (p.n + p.nt - 1) / p.nt * tiles_m;
+            table.end[0]   = linear_cover(p.n, p.nt) * tiles_m;
         }
         __syncwarp();
         if (warp == 0)

@@ -332,8 +332,9 @@ void spmm_b200_decompose_v1(const uint16_t* A, uint16_t* A1, uint16_t* A2, int l
  *
  * All calls are asynchronous on `stream`, allocate nothing and may be captured in a CUDA graph (make the first
  * call on a device outside a capture, as for the SpMM).  A, B, codes and workspaces start on 16-byte boundaries.
- * N = 0 returns at once.  They return a cudaError_t as an int; cudaErrorInvalidValue for sizes, types or
- * pointers that are not as described here, before anything is launched. */
+ * N = 0 returns at once.  N is at most 2^31 - 513, K at most 2^29 (8 bits) or 2^27 (16 bits), and the tiles of 128 or 256
+ * features by 16 to 256 tokens, times the groups, have to be fewer than 2^31.  The calls return a cudaError_t as an int;
+ * cudaErrorInvalidValue for sizes, types or pointers that are not as described here, before anything is launched. */
 #define SPMM_B200_FP16 0
 #define SPMM_B200_BF16 1
 

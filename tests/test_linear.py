@@ -84,3 +84,20 @@ def test_c_boundary_refuses_before_any_cuda_call(sp):
         args = list(good)
         args[at] = value
         assert grouped8(None, *args) == 1, (at, value)
+
+
+def test_sizes_that_indices_cannot_hold_are_refused(sp):
+    """The last tile's columns have to have numbers that fit an int, and a row of K byte offsets that do; a 16-bit depth is
+    one accumulation, which has to end before a wait gives up."""
+    lib, p = sp.spmm_api.LIB, ctypes.c_void_p(4096)
+    most = 2 ** 31 - 513
+    for n in (most + 1, 2 ** 31 - 256, 2 ** 31 - 1):
+        assert sp.linear_workspace_bytes(1, 128, n, 16, True) == 0
+        assert sp.linear_workspace_bytes(3, 128, n, 16, False) == 0
+        assert lib.spmm_b200_fp8_linear(None, p, p, p, p, p, 0, 128, n, 16, None, 0) == 1
+        assert lib.spmm_b200_grouped_linear(None, p, p, p, 0, p, 3, 128, n, 16, None, 0) == 1
+        assert lib.spmm_b200_grouped_fp8_linear(None, p, p, p, p, p, 0, p, 3, 128, n, 16, None, 0) == 1
+    for n, k, eight, fits in [(most, 16, True, True), (most, 16, False, True), (16, 2 ** 29, True, True), (16, 2 ** 29 + 16, True, False),
+                              (16, 2 ** 27, False, True), (16, 2 ** 27 + 8, False, False)]:
+        assert (sp.linear_workspace_bytes(1, 128, n, k, eight) > 0) == fits, (n, k, eight)
+    assert lib.spmm_b200_grouped_linear(None, p, p, p, 0, p, 3, 128, 16, 2 ** 27 + 8, None, 0) == 1

@@ -473,3 +473,29 @@ def test_python_refusals(sp):
     small = torch.zeros(64, dtype=torch.uint8, device="cuda")  # too small a workspace is not used
     assert sp.fp8_linear(None, a, sa, b, sb, c, m, n, k, small) == 0
     assert not bool(small.any())
+
+
+@pytest.mark.parametrize("eight", [True, False], ids=["e4m3", "fp16"])
+def test_as_many_tokens_as_there_may_be(sp, eight):
+    """2^31 - 513 tokens of the smallest depth, in one group but for a few: counts and widths of tiles near the end of an
+    int.  Values 0, 1 and 128, whose sums (16 of them at most) are exact in fp16."""
+    m, n, k = 1, 2 ** 31 - 513, 16 if eight else 8
+    free = torch.cuda.mem_get_info()[0]
+    if free < 64 << 30:
+        pytest.skip("needs 64 GB of device memory, %d GB are free" % (free >> 30))
+    bits = 0x38 if eight else 0x3c00  # 1.0; twice the bits are 128 (e4m3), 2^15 would be too much for fp16: halves take 0 and 1
+    b = torch.randint(0, 3 if eight else 2, (n, k), dtype=torch.uint8 if eight else torch.int16, device="cuda", generator=rng(n, k))
+    b.mul_(bits)
+    b = b.view(torch.float8_e4m3fn if eight else torch.float16)
+    a = torch.ones((2, m, k), device="cuda").to(b.dtype)
+    c = torch.full((n, m), 7.0, dtype=torch.float16, device="cuda")
+    off = torch.tensor([2, 7, n - 1], dtype=torch.int32, device="cuda")
+    sa = sb = None
+    if eight:
+        sa, sb = torch.ones((2, 1, 1), device="cuda"), torch.ones((1, n), device="cuda")
+    assert call(sp, a, sa, b, sb, c, off, 2, m, n, k, None) == 0
+    assert sp.device_status() == 0
+    assert bool((c[:2] == 7).all()) and bool((c[n - 1] == 7).all())
+    for first in range(2, n - 1, 1 << 26):
+        last = min(n - 1, first + (1 << 26))
+        assert torch.equal(c[first:last, 0], b[first:last].to(torch.float16).sum(1)), first
