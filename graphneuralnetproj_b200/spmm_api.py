@@ -327,6 +327,12 @@ def _blocks(n):
     return -(-n // 128)
 
 
+def _check_sizes(sizes):
+    """sizes: the bitwise or of a call's sizes.  The C boundary takes ints, and a longer one would arrive as its last 32 bits."""
+    if sizes >> 31:
+        raise ValueError("sizes must be 0 .. 2^31 - 1")
+
+
 def quantize_fp8(stream, X, codes, scales, block_rows):
     """e4m3 codes and fp32 scales of X ([rows][cols], or [groups][rows][cols] for block_rows = 128), fp16 or bf16.
 
@@ -337,6 +343,7 @@ def quantize_fp8(stream, X, codes, scales, block_rows):
         raise ValueError("X must be [rows][cols], or [groups][rows][cols] with block_rows = 128; block_rows 1 or 128")
     groups = X.shape[0] if X.dim() == 3 else 1
     rows, cols = X.shape[-2:]
+    _check_sizes(groups | rows | cols)
     blocks = _blocks(cols) * (rows if block_rows == 1 else groups * _blocks(rows))
     device, handle = _launch_on(stream)
     elements = X.numel()
@@ -346,7 +353,10 @@ def quantize_fp8(stream, X, codes, scales, block_rows):
 
 
 def linear_workspace_bytes(groups, M_Global, N_Global, K_Global, eight_bit):
-    """Bytes of (once zero-filled) workspace for fp8_linear (groups = 1), grouped_linear and grouped_fp8_linear."""
+    """Bytes of (once zero-filled) workspace for fp8_linear (groups = 1), grouped_linear and grouped_fp8_linear; 0 for sizes
+    that they refuse."""
+    if (groups | M_Global | N_Global | K_Global) >> 31:
+        return 0
     return int(LIB.spmm_b200_linear_workspace_bytes(groups, M_Global, N_Global, K_Global, int(eight_bit)))
 
 
@@ -355,6 +365,7 @@ def fp8_linear(stream, A, A_scales, B, B_scales, C, M_Global, N_Global, K_Global
     activations: block_rows = 1); C fp16 or bf16.  workspace: a CUDA tensor, zero-filled once, of
     linear_workspace_bytes(1, M, N, K, True) bytes, or None.  Returns a cudaError_t as an int; asynchronous."""
     M, N, K = M_Global, N_Global, K_Global
+    _check_sizes(M | N | K)
     device, handle = _launch_on(stream)
     ws, ws_bytes = _workspace(workspace, device)
     return LIB.spmm_b200_fp8_linear(handle, _operand("A", A, device, _Torch.codes, M * K),
@@ -369,6 +380,7 @@ def grouped_linear(stream, A, B, C, group_offsets, groups, M_Global, N_Global, K
     device); A[groups][M][K], B[N][K], C[N][M], all fp16 or all bf16.  Rows of C outside all groups stay as they were.
     workspace: linear_workspace_bytes(groups, M, N, K, False) bytes, zero-filled once, or None."""
     M, N, K = M_Global, N_Global, K_Global
+    _check_sizes(groups | M | N | K)
     if B.dtype is not A.dtype or C.dtype is not A.dtype:
         raise ValueError("A, B and C must have the same type")
     device, handle = _launch_on(stream)
@@ -383,6 +395,7 @@ def grouped_fp8_linear(stream, A, A_scales, B, B_scales, C, group_offsets, group
     """grouped_linear from e4m3 codes and scales: A[groups][M][K] with A_scales[groups][ceil(M / 128)][ceil(K / 128)],
     B[N][K] with B_scales[ceil(K / 128)][N]; C fp16 or bf16."""
     M, N, K = M_Global, N_Global, K_Global
+    _check_sizes(groups | M | N | K)
     device, handle = _launch_on(stream)
     ws, ws_bytes = _workspace(workspace, device)
     return LIB.spmm_b200_grouped_fp8_linear(handle, _operand("A", A, device, _Torch.codes, groups * M * K),

@@ -101,3 +101,26 @@ def test_sizes_that_indices_cannot_hold_are_refused(sp):
                               (16, 2 ** 27, False, True), (16, 2 ** 27 + 8, False, False)]:
         assert (sp.linear_workspace_bytes(1, 128, n, k, eight) > 0) == fits, (n, k, eight)
     assert lib.spmm_b200_grouped_linear(None, p, p, p, 0, p, 3, 128, 16, 2 ** 27 + 8, None, 0) == 1
+
+
+def test_python_sizes_longer_than_an_int_are_refused(sp):
+    """2^32 + 128 would arrive at the C boundary as 128."""
+    import torch
+    far = 2 ** 32 + 128
+    for at in range(4):
+        sizes = [1, 128, 16, 128]
+        assert sp.linear_workspace_bytes(*sizes, True) > 0
+        sizes[at] = far
+        assert sp.linear_workspace_bytes(*sizes, True) == 0
+        t = torch.zeros((16, 128), dtype=torch.bfloat16)
+        if at > 0:
+            with pytest.raises(ValueError, match="sizes"):
+                sp.fp8_linear(None, t, t, t, t, t, *sizes[1:], None)
+        with pytest.raises(ValueError, match="sizes"):
+            sp.grouped_linear(None, t, t, t, t, *sizes, None)
+        with pytest.raises(ValueError, match="sizes"):
+            sp.grouped_fp8_linear(None, t, t, t, t, t, t, *sizes, None)
+    with pytest.raises(ValueError, match="sizes"):
+        sp.quantize_fp8(None, torch.zeros((far, 0, 16), dtype=torch.bfloat16), t, t, 128)
+    with pytest.raises(ValueError, match="sizes"):
+        sp.fp8_linear(None, t, t, t, t, t, 128, -1, 128, None)
