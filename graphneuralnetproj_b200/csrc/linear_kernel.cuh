@@ -498,11 +498,15 @@ linear_kernel(const __grid_constant__ LinearParams p)
                     return false;
                 const float* sa = p.a_scales + (static_cast<size_t>(next_tile.group) * tiles_m + next_tile.m0 / kLinearRows) * p.kb;
                 const int    k0 = next_k * kStepBlocks;
-                f.a             = __ldg(sa + min(k0 + (lane & (kGroupBlocks - 1)), p.kb - 1));
+                // A k-block behind the end of K, the second of the last step, has the factor 0: a product of zeros times an
+                // infinite scale of the block before it would be NaN.
+                const int own = k0 + (lane & (kGroupBlocks - 1));
+                f.a           = own < p.kb ? __ldg(sa + own) : 0.0f;
 #pragma unroll
                 for (int j = 0; j < PER; j++) {
-                    const int v = lane + 32 * j, block = min(k0 + (v >> acc_shift), p.kb - 1), column = v & (acc_width - 1);
-                    f.b[j] = __ldg(p.b_scales + static_cast<size_t>(block) * p.n + next_tile.row0 + min(column, next_tile.rows - 1));
+                    const int v = lane + 32 * j, block = k0 + (v >> acc_shift), column = v & (acc_width - 1);
+                    f.b[j] = block < p.kb ? __ldg(p.b_scales + static_cast<size_t>(block) * p.n + next_tile.row0 + min(column, next_tile.rows - 1))
+                                          : 0.0f;
                 }
                 next_k += group_steps;
                 if (next_k >= next_seg.kb1) {

@@ -499,3 +499,31 @@ def test_as_many_tokens_as_there_may_be(sp, eight):
     for first in range(2, n - 1, 1 << 26):
         last = min(n - 1, first + (1 << 26))
         assert torch.equal(c[first:last, 0], b[first:last].to(torch.float16).sum(1)), first
+
+
+@pytest.mark.parametrize("kb", [1, 3, 4, 7], ids=lambda kb: "%d-blocks" % kb)
+@pytest.mark.parametrize("n", [1, 20, 50, 100, 300])
+def test_infinite_scales_at_the_end_of_k(sp, n, kb):
+    """Infinite scales of the last k-block give what the formula gives, whether the number of k-blocks is odd or even: codes
+    are positive, so it is an infinity, and NaN for the scale that is NaN."""
+    m, k = 264, 128 * kb - 48
+    a = torch.full((1, m, k), 0x38, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    b = torch.full((n, k), 0x40, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    sa, sb = torch.full((1, kb_of(m), kb), 0.25, device="cuda"), torch.full((kb, n), 0.5, device="cuda")
+    sa[0, 1, kb - 1] = float("inf")
+    sb[kb - 1, n // 2] = float("-inf")
+    sb[kb - 1, n // 3] = float("nan")
+    depth = torch.full((kb,), 128.0, dtype=torch.float64, device="cuda")
+    depth[kb - 1] = 80
+    want = 2 * torch.einsum("b,ob,bn->no", depth, sa[0].double(), sb.double()).repeat_interleave(128, 1)[:, :m]
+    assert bool(want.isinf().any()) or n < 3
+    for groups in (None, [0, n // 2, n]):
+        c = torch.full((n, m), 7.0, dtype=torch.bfloat16, device="cuda")
+        off = None if groups is None else torch.tensor(groups, dtype=torch.int32, device="cuda")
+        count = 1 if groups is None else 2
+        assert call(sp, a.expand(count, -1, -1).contiguous(), sa.repeat(count, 1, 1), b, sb, c, off, count, m, n, k,
+                    workspace_for(sp, count, m, n, k, True)) == 0
+        finite = want.isfinite()
+        assert torch.equal(c[~finite].double().nan_to_num(nan=5.0), want[~finite].nan_to_num(nan=5.0))
+        assert bool(((c[finite].double() - want[finite]).abs() <= HALF_STEP[torch.bfloat16] * want[finite].abs()).all())
+    assert sp.device_status() == 0
