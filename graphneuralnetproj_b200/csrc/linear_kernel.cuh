@@ -24,6 +24,9 @@
 // MMAs, commits and TMA loads are issued by an elected lane in code that is uniform for the compiler (values that come out of
 // shared memory pass through linear_uniform): under `lane == 0` four MMAs and two commits took 520 cycles, now 170.
 //
+// A launch starts before its predecessor in the stream has finished, which may be what writes the group borders and the scales:
+// they are read through L2 (__ldcg), never through the non-coherent path, whose data must not change while a kernel runs.
+//
 // Roles: warp 0 TMA, warp 1 MMA issue and TMEM, warp 2 scales, warps 4..11 epilogue (warp % 4 = quarter of the TMEM
 // lanes, warp / 4 - 1 = every other chunk of columns).  Every wait is bounded; a block that gives up records it.
 #pragma once
@@ -169,8 +172,8 @@ linear_build_table(const LinearParams& p, const LinearTable& table, int* warp_su
     for (int e = e0; e < e1; e++) {
         int from = 0, rows = p.n;
         if (p.offsets) {
-            from = min(max(__ldg(p.offsets + e), 0), p.n);
-            rows = max(min(max(__ldg(p.offsets + e + 1), 0), p.n) - from, 0);
+            from = min(max(__ldcg(p.offsets + e), 0), p.n);
+            rows = max(min(max(__ldcg(p.offsets + e + 1), 0), p.n) - from, 0);
         }
         table.row[e]   = from;
         table.rows[e]  = rows;
@@ -501,11 +504,11 @@ linear_kernel(const __grid_constant__ LinearParams p)
                 // A k-block behind the end of K, the second of the last step, has the factor 0: a product of zeros times an
                 // infinite scale of the block before it would be NaN.
                 const int own = k0 + (lane & (kGroupBlocks - 1));
-                f.a           = own < p.kb ? __ldg(sa + own) : 0.0f;
+                f.a           = own < p.kb ? __ldcg(sa + own) : 0.0f;
 #pragma unroll
                 for (int j = 0; j < PER; j++) {
                     const int v = lane + 32 * j, block = k0 + (v >> acc_shift), column = v & (acc_width - 1);
-                    f.b[j] = block < p.kb ? __ldg(p.b_scales + static_cast<size_t>(block) * p.n + next_tile.row0 + min(column, next_tile.rows - 1))
+                    f.b[j] = block < p.kb ? __ldcg(p.b_scales + static_cast<size_t>(block) * p.n + next_tile.row0 + min(column, next_tile.rows - 1))
                                           : 0.0f;
                 }
                 next_k += group_steps;

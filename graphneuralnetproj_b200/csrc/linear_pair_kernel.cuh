@@ -218,14 +218,14 @@ linear_pair_kernel(const __grid_constant__ LinearParams p)
                 if (next_seg.tile < 0)
                     return false;
                 const int m_block = min(next_tile.m0 / kLinearRows + ((lane >> 2) & 1), blocks_m - 1);
-                a = __ldg(p.a_scales + (static_cast<size_t>(next_tile.group) * blocks_m + m_block) * p.kb
+                a = __ldcg(p.a_scales + (static_cast<size_t>(next_tile.group) * blocks_m + m_block) * p.kb
                           + min(next_k + mine + (lane & 3), p.kb - 1));
 #pragma unroll
                 for (int u = 0; u < PER; u++) {
                     const float* from = p.b_scales + static_cast<size_t>(min(next_k + mine + u, p.kb - 1)) * p.n + next_tile.row0;
 #pragma unroll
                     for (int j = 0; j < 4; j++)
-                        b[u][j] = __ldg(from + min(static_cast<int>(rank) * kLinearRows + lane + 32 * j, next_tile.rows - 1));
+                        b[u][j] = __ldcg(from + min(static_cast<int>(rank) * kLinearRows + lane + 32 * j, next_tile.rows - 1));
                 }
                 next_k += kPairBatch;
                 if (next_k >= next_seg.kb1) {

@@ -267,6 +267,18 @@ __device__ __forceinline__ uint4 ld_stream_128(const uint4* p)
     return v;
 }
 
+// The same for data that may have been written since this kernel started (by its predecessor in the stream, until
+// grid_dependency_wait returns): the non-coherent path above may not be used for that.
+__device__ __forceinline__ uint4 ld_once_128(const uint4* p)
+{
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p)
+                 : "memory");
+    return v;
+}
+
 __device__ __forceinline__ void st_shared_zero_128(uint32_t addr)
 {
     asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0u) : "memory");

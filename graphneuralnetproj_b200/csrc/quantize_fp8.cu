@@ -178,7 +178,7 @@ quantize_rows_kernel(const uint4* __restrict__ x, uint4* __restrict__ codes, flo
         for (int i = 0; i < 2; i++)
 #pragma unroll
             for (int h = 0; h < 2; h++)
-                v[i][h] = first + 32 * i < per_row ? ptx::ld_stream_128(x + 2 * (base + 32 * i) + h) : make_uint4(0, 0, 0, 0);
+                v[i][h] = first + 32 * i < per_row ? ptx::ld_once_128(x + 2 * (base + 32 * i) + h) : make_uint4(0, 0, 0, 0);
         // amax of the lane's two blocks, one per half of a register
         auto amax_of = [&](bool only_finite) {
             uint32_t m[2];
@@ -240,7 +240,7 @@ quantize_blocks_kernel(const uint4* __restrict__ x, uint4* __restrict__ codes, f
     for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int h = 0; h < 2; h++)
-            v[i][h] = col < per_row && row0 + 32 * i < rows ? ptx::ld_stream_128(x + 2 * (base + static_cast<size_t>(32 * i) * per_row) + h)
+            v[i][h] = col < per_row && row0 + 32 * i < rows ? ptx::ld_once_128(x + 2 * (base + static_cast<size_t>(32 * i) * per_row) + h)
                                                             : make_uint4(0, 0, 0, 0);
     auto amax_of = [&](bool only_finite) {
         uint32_t m = 0;

@@ -527,3 +527,52 @@ def test_infinite_scales_at_the_end_of_k(sp, n, kb):
         assert torch.equal(c[~finite].double().nan_to_num(nan=5.0), want[~finite].nan_to_num(nan=5.0))
         assert bool(((c[finite].double() - want[finite]).abs() <= HALF_STEP[torch.bfloat16] * want[finite].abs()).all())
     assert sp.device_status() == 0
+
+
+def test_chain_of_calls_on_buffers_written_just_ahead(sp):
+    """Quantiser, product, quantiser, experts back to back, every launch starting while the one that writes its operands,
+    scales or group borders may still run, all in buffers that the turn before has used with other values: the same as with the
+    device idle between the calls."""
+    n, hidden, inner, groups, turns = 24, 1024, 1536, 3, 12
+    g = rng(5)
+    w1, s1, _, _, _, _ = random_operands(1, inner, 1, hidden, None, 1)
+    w2, s2, _, _, _, _ = random_operands(groups, hidden, 1, inner, None, 2)
+    w3 = torch.randn((groups, hidden, hidden), device="cuda", generator=g).mul_(0.05).to(torch.bfloat16)
+    inputs = [torch.randn((n, hidden), device="cuda", generator=g).mul_(2.0 ** (t % 5)).to(torch.bfloat16) for t in range(turns)]
+    tables = [torch.tensor([t % 3, 5 + t % 7, 20 - t % 8, n - t % 2], dtype=torch.int32, device="cuda") for t in range(turns)]
+    ws = torch.zeros(max(sp.linear_workspace_bytes(e, inner, n, inner, True) for e in (1, groups)), dtype=torch.uint8, device="cuda")
+    x, off = torch.empty_like(inputs[0]), torch.empty_like(tables[0])
+    c1, c2, c3 = (torch.empty((n, m), dtype=torch.bfloat16, device="cuda") for m in (inner, hidden, hidden))
+    codes = [torch.empty((n, k), dtype=torch.float8_e4m3fn, device="cuda") for k in (hidden, inner)]
+    scales = [torch.empty((kb_of(k), n), device="cuda") for k in (hidden, inner)]
+
+    def turn(t, idle, keep):
+        steps = [lambda: x.copy_(inputs[t]) is None, lambda: off.copy_(tables[t]) is None, lambda: c2.zero_() is None, lambda: c3.zero_() is None,
+                 lambda: sp.quantize_fp8(None, x, codes[0], scales[0], 1),
+                 lambda: sp.fp8_linear(None, w1, s1, codes[0], scales[0], c1, inner, n, hidden, ws),
+                 lambda: sp.quantize_fp8(None, c1, codes[1], scales[1], 1),
+                 lambda: sp.grouped_fp8_linear(None, w2, s2, codes[1], scales[1], c2, off, groups, hidden, n, inner, ws),
+                 lambda: sp.grouped_linear(None, w3, c2, c3, off, groups, hidden, n, hidden, ws)]
+        for step in steps:
+            assert step() == 0
+            if idle:
+                torch.cuda.synchronize()
+        keep[t].copy_(c3)
+
+    want, got, replayed = (torch.empty((turns, n, hidden), dtype=torch.bfloat16, device="cuda") for _ in range(3))
+    for t in range(turns):
+        turn(t, True, want)
+    for _ in range(3):
+        for t in range(turns):
+            turn(t, False, got)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for t in range(turns):
+            turn(t, False, replayed)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert sp.device_status() == 0
+    assert bool(want.isfinite().all()) and bool((want != 0).any(2).any(1).all())
+    assert torch.equal(want, got) and torch.equal(want, replayed)
