@@ -254,6 +254,26 @@ LinearShape shape_of(bool eight, bool ragged, int groups, int m, int n, int k)
 
 }  // namespace
 
+// Two warps wait for a phase of a barrier that nothing completes: the first to reach the limit gives up, the other follows its
+// abort word, each as a whole (the vote after the wait takes part of all lanes), and the block ends normally.
+__global__ void linear_wait_that_runs_out_kernel(uint64_t limit_ns)
+{
+    __shared__ __align__(8) uint64_t bar;
+    __shared__ int                   abort_word;
+    if (threadIdx.x == 0) {
+        ptx::mbar_init(ptx::smem_addr(&bar), 1);
+        ptx::mbar_init_fence();
+        abort_word = 0;
+    }
+    __syncthreads();
+    // warp 1 alone could wait as long as any wait of the kernels
+    const bool ok = linear_wait(ptx::smem_addr(&bar), 0, &abort_word, threadIdx.x < 32 ? limit_ns : ptx::kWaitLimitNs);
+    const bool all_gave_up = __all_sync(0xffffffffu, !ok);
+    __syncthreads();
+    if (threadIdx.x == 32 && all_gave_up && abort_word != 0)
+        atomicExch(&g_linear_status, 1);
+}
+
 int linear_status(int reset)
 {
     int         status = 0;
@@ -343,6 +363,15 @@ int spmm_b200_grouped_fp8_linear(void*        stream,
     using namespace spmm_b200;
     return static_cast<int>(linear(static_cast<cudaStream_t>(stream), shape_of(true, true, groups, M_Global, N_Global, K_Global), A, A_scales,
                                    B, B_scales, C, C_type, group_offsets, workspace, workspace_bytes));
+}
+
+int spmm_b200_selftest_linear_wait_timeout(void* stream, unsigned int limit_ms)
+{
+    if (limit_ms == 0 || limit_ms > 1000)
+        return static_cast<int>(cudaErrorInvalidValue);
+    spmm_b200::linear_wait_that_runs_out_kernel<<<1, 64, 0, static_cast<cudaStream_t>(stream)>>>(
+        static_cast<uint64_t>(limit_ms) * 1000000ull);
+    return static_cast<int>(cudaGetLastError());
 }
 
 int spmm_b200_linear_plan(int tiles, int kb, int workers, int overhead, int pieces, int worker, int index, int* segment)

@@ -278,28 +278,33 @@ SPMM_B200_HD int linear_group_steps(int nt)
     return nt <= 32 ? 4 : (nt <= 64 ? 2 : 1);
 }
 
-// A bounded wait of all lanes of a warp, or of one.  Parked at once: here most waits are long, and the polling of ten warps
-// slows the others down (64 experts of 2048 x 4096 in bf16: 130 us with 64 polls before parking, 121 without).
-__device__ __forceinline__ bool linear_wait(uint32_t bar, uint32_t parity, volatile int* abort_word)
+// A bounded wait of a whole warp, with the same answer for all of its lanes: warp-wide instructions follow, and a lane that gave
+// up while the others saw the phase complete would leave them waiting for it.  The phase cannot pass before all lanes have seen it,
+// since the next one needs this warp.  Parked at once: here most waits are long, and the polling of ten warps slows the
+// others down (64 experts of 2048 x 4096 in bf16: 130 us with 64 polls before parking, 121 without).
+__device__ __forceinline__ bool linear_wait(uint32_t bar, uint32_t parity, volatile int* abort_word, uint64_t limit_ns = ptx::kWaitLimitNs)
 {
     uint64_t start = 0;
 #pragma unroll 1
     for (uint32_t polls = 0;; polls++) {
-        if (ptx::mbar_try_wait_suspend(bar, parity, ptx::kSuspendNs))
+        if (__all_sync(0xffffffffu, ptx::mbar_try_wait_suspend(bar, parity, ptx::kSuspendNs)))
             return true;
-        if (*abort_word != 0)
-            return false;
+        bool give_up = *abort_word != 0;
         if ((polls & 255u) == 0) {
             const uint64_t now = ptx::global_timer_ns();
             if (start == 0)
                 start = now;
-            else if (now - start > ptx::kWaitLimitNs) {
+            else if (now - start > limit_ns) {
                 *abort_word = 1;
-                return false;
+                give_up     = true;
             }
         }
+        if (__any_sync(0xffffffffu, give_up))
+            return false;
     }
 }
+
+constexpr uint64_t kDrainNs = 10000000ull;  // an abandoned block waits so long at most for each copy or product under way
 
 template<bool EIGHT>
 __global__ void __launch_bounds__(kLinearThreads, 1)
@@ -326,7 +331,8 @@ linear_kernel(const __grid_constant__ LinearParams p)
     auto empty      = [&](int s) { return bar_base + 8u * (kLinearMaxStages + s); };
     auto acc_full   = [&](int b) { return bar_base + 8u * (2 * kLinearMaxStages + b); };
     auto acc_free   = [&](int b) { return bar_base + 8u * (2 * kLinearMaxStages + BUFS + b); };
-    constexpr uint32_t kWords = 8u * (2 * kLinearMaxStages + 2 * BUFS);
+    const uint32_t     drained = bar_base + 8u * (2 * kLinearMaxStages + 2 * BUFS);
+    constexpr uint32_t kWords  = 8u * (2 * kLinearMaxStages + 2 * BUFS + 1);
     static_assert(kWords + 64 <= 512, "barrier block");
     volatile uint32_t* tmem_slot  = reinterpret_cast<volatile uint32_t*>(smem + bar_off + kWords);
     volatile int*      abort_word = reinterpret_cast<volatile int*>(smem + bar_off + kWords + 4);
@@ -345,6 +351,7 @@ linear_kernel(const __grid_constant__ LinearParams p)
             ptx::mbar_init(acc_full(b), EIGHT ? 2 : 1);  // the products, and the scales
             ptx::mbar_init(acc_free(b), kEpilogueTeams);
         }
+        ptx::mbar_init(drained, 1);
         *abort_word = 0;
         ptx::mbar_init_fence();
     }
@@ -693,15 +700,22 @@ linear_kernel(const __grid_constant__ LinearParams p)
     }
 
     // ---------------------------------------------------------------- exit
-    __syncwarp();
-    if (warp == 0 && *abort_word != 0)  // copies still under way land before the block's memory goes
-        for (int i = max(0, issued - p.stages); i < issued; i++)
-            ptx::mbar_wait_quiet(full(i % p.stages), (i / p.stages) & 1, 10000000ull);
     ptx::tc_fence_before_sync();
     __syncthreads();
-    if (threadIdx.x == 0 && *abort_word != 0)
+    const bool abandoned = *abort_word != 0;
+    if (threadIdx.x == 0 && abandoned)
         atomicExch(&g_linear_status, 1);
+    if (warp == 0 && abandoned)  // copies still under way land before the block's memory goes
+        for (int i = max(0, issued - p.stages); i < issued; i++)
+            ptx::mbar_wait_quiet(full(i % p.stages), (i / p.stages) & 1, kDrainNs);
     if (warp == 1) {
+        if (abandoned) {  // and products end before TMEM does
+            if (ptx::elect_one())
+                ptx::umma_commit(drained);
+            __syncwarp();
+            ptx::mbar_wait_quiet(drained, 0, kDrainNs);
+            __syncwarp();
+        }
         ptx::tc_fence_after_sync();
         ptx::tmem_dealloc(tmem_base, 512);
     }

@@ -58,7 +58,8 @@ linear_pair_kernel(const __grid_constant__ LinearParams p)
     auto acc_free = [&](int b) { return bar_base + 8u * (2 * kPairStages + 2 + b); };  // the leader's
     auto scale_full = [&](int b) { return bar_base + 8u * (2 * kPairStages + 4 + b); };  // each block's own
     auto scale_free = [&](int b) { return bar_base + 8u * (2 * kPairStages + 6 + b); };
-    constexpr uint32_t kWords = 8u * (2 * kPairStages + 8);
+    const uint32_t     drained = bar_base + 8u * (2 * kPairStages + 8);
+    constexpr uint32_t kWords  = 8u * (2 * kPairStages + 9);
     volatile uint32_t* tmem_slot  = reinterpret_cast<volatile uint32_t*>(smem + bar_off + kWords);
     volatile int*      abort_word = reinterpret_cast<volatile int*>(smem + bar_off + kWords + 4);
     int* const         warp_sums  = reinterpret_cast<int*>(smem + bar_off + kWords + 8);
@@ -80,6 +81,7 @@ linear_pair_kernel(const __grid_constant__ LinearParams p)
             ptx::mbar_init(scale_full(b), 2);
             ptx::mbar_init(scale_free(b), EPI);
         }
+        ptx::mbar_init(drained, 1);
         *abort_word = 0;
         ptx::mbar_init_fence();
     }
@@ -459,14 +461,23 @@ linear_pair_kernel(const __grid_constant__ LinearParams p)
     }
 
     // ---------------------------------------------------------------- exit
-    __syncwarp();
-    if (warp == 0 && rank == 0 && *abort_word != 0)  // both blocks' copies still under way are counted here
-        for (int i = max(0, issued - p.stages); i < issued; i++)
-            ptx::mbar_wait_quiet(full(i % p.stages), (i / p.stages) & 1, 10000000ull);
     ptx::tc_fence_before_sync();
     __syncthreads();
-    if (threadIdx.x == 0 && *abort_word != 0)
+    const bool abandoned = *abort_word != 0;
+    if (threadIdx.x == 0 && abandoned)
         atomicExch(&g_linear_status, 1);
+    if (abandoned && rank == 0 && warp == 0)  // both blocks' copies still under way are counted here
+        for (int i = max(0, issued - p.stages); i < issued; i++)
+            ptx::mbar_wait_quiet(full(i % p.stages), (i / p.stages) & 1, kDrainNs);
+    if (abandoned && rank == 0 && warp == 1) {  // and products end before TMEM does
+        if (ptx::elect_one())
+            ptx::umma_commit_pair(ptx::map_to_cta(drained, 0));
+        __syncwarp();
+        ptx::mbar_wait_quiet(drained, 0, kDrainNs);
+        __syncwarp();
+    }
+    if (abandoned && rank == 1 && warp == 0)  // copies that the leader no longer counts: it has given up on them
+        ptx::mbar_wait_quiet(drained, 0, kDrainNs);  // of this block: nothing arrives on it
     // Neither block leaves while its partner may still arrive on its barriers or the leader's MMAs read its memory.
     ptx::cluster_sync_all();
     if (warp == 1) {

@@ -99,6 +99,8 @@ def _load():
     lib.spmm_b200_device_status.restype = ctypes.c_int
     lib.spmm_b200_selftest_wait_timeout.argtypes = [ctypes.c_void_p, ctypes.c_uint]
     lib.spmm_b200_selftest_wait_timeout.restype = ctypes.c_int
+    lib.spmm_b200_selftest_linear_wait_timeout.argtypes = [ctypes.c_void_p, ctypes.c_uint]
+    lib.spmm_b200_selftest_linear_wait_timeout.restype = ctypes.c_int
     lib.spmm_b200_synth_fp16.argtypes = [_u16p, ctypes.c_long, ctypes.c_uint64, ctypes.c_double, ctypes.c_double]
     lib.spmm_b200_synth_fp16.restype = None
     lib.spmm_b200_synth_fp16_block.argtypes = [_u16p] + [ctypes.c_long] * 5 + [ctypes.c_uint64, ctypes.c_double, ctypes.c_double]
@@ -532,6 +534,12 @@ def selftest_wait_timeout(limit_ms=50):
     """Launches a wait that nothing satisfies; device_status() must report 1 afterwards (then reset it)."""
     import torch
     return int(LIB.spmm_b200_selftest_wait_timeout(ctypes.c_void_p(torch.cuda.current_stream().cuda_stream), limit_ms))
+
+
+def selftest_linear_wait_timeout(limit_ms=50):
+    """The same for the wait of the linear-layer kernels."""
+    import torch
+    return int(LIB.spmm_b200_selftest_linear_wait_timeout(ctypes.c_void_p(torch.cuda.current_stream().cuda_stream), limit_ms))
 
 
 def synth_fp16(shape, seed, sigma, p_zero=0.0):

@@ -419,6 +419,9 @@ int spmm_b200_device_status(int reset);
  * spmm_b200_device_status() then reports 1 until it is reset.  No counterpart in the reference. */
 int spmm_b200_selftest_wait_timeout(void* stream, unsigned int limit_ms);
 
+/* The same for the wait of the linear-layer kernels and the status word that they report through. */
+int spmm_b200_selftest_linear_wait_timeout(void* stream, unsigned int limit_ms);
+
 /* Seeded synthetic inputs (stand-ins for pruned model weights and
  * activations): element i of the stream is drawn from a counter-based
  * splitmix64 generator, value = fp16(sigma * gaussian), zeroed with

@@ -124,3 +124,8 @@ def test_python_sizes_longer_than_an_int_are_refused(sp):
         sp.quantize_fp8(None, torch.zeros((far, 0, 16), dtype=torch.bfloat16), t, t, 128)
     with pytest.raises(ValueError, match="sizes"):
         sp.fp8_linear(None, t, t, t, t, t, 128, -1, 128, None)
+
+
+def test_wait_selftest_refuses_limits_out_of_range(sp):
+    for limit_ms in (0, 1001, 2 ** 32 - 1):
+        assert sp.spmm_api.LIB.spmm_b200_selftest_linear_wait_timeout(None, limit_ms) == 1

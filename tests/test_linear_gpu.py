@@ -576,3 +576,16 @@ def test_chain_of_calls_on_buffers_written_just_ahead(sp):
     assert sp.device_status() == 0
     assert bool(want.isfinite().all()) and bool((want != 0).any(2).any(1).all())
     assert torch.equal(want, got) and torch.equal(want, replayed)
+
+
+def test_a_wait_that_runs_out_is_reported_and_cleared(sp):
+    """Failure detection without a fault: two warps wait with the linear layers' bounded wait for something that nothing does.
+    One gives up after 50 ms, the other follows, the block ends, the status word says so until it is reset, and the
+    layers keep working."""
+    assert sp.device_status(reset=True) == 0
+    assert sp.selftest_linear_wait_timeout(50) == 0
+    assert sp.device_status() == 1
+    assert sp.device_status(reset=True) == 1
+    assert sp.device_status() == 0
+    for n in (20, 300):
+        run_case(sp, 1, 264, n, 528, None, torch.float16, None, True, integer_operands, True)
