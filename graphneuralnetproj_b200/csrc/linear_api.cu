@@ -189,7 +189,9 @@ cudaError_t launch(cudaStream_t stream, LinearParams& p, const LinearShape& s)
     }
     config.gridDim = dim3(PAIR ? 2 * workers : workers);
     e              = cudaLaunchKernelEx(&config, kern, p);
-    return e != cudaSuccess ? e : cudaGetLastError();
+    if (e != cudaSuccess)
+        (void)cudaGetLastError();
+    return e;  // not what an earlier call has left behind
 }
 
 cudaError_t linear(cudaStream_t stream, LinearShape s, const void* A, const float* A_scales, const void* B, const float* B_scales, void* C,
@@ -278,8 +280,10 @@ int linear_status(int reset)
 {
     int         status = 0;
     cudaError_t e      = cudaMemcpyFromSymbol(&status, g_linear_status, sizeof(int));
-    if (e != cudaSuccess)
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();
         return -static_cast<int>(e);
+    }
     if (reset) {
         const int zero = 0;
         cudaMemcpyToSymbol(g_linear_status, &zero, sizeof(int));
@@ -369,9 +373,14 @@ int spmm_b200_selftest_linear_wait_timeout(void* stream, unsigned int limit_ms)
 {
     if (limit_ms == 0 || limit_ms > 1000)
         return static_cast<int>(cudaErrorInvalidValue);
-    spmm_b200::linear_wait_that_runs_out_kernel<<<1, 64, 0, static_cast<cudaStream_t>(stream)>>>(
-        static_cast<uint64_t>(limit_ms) * 1000000ull);
-    return static_cast<int>(cudaGetLastError());
+    cudaLaunchConfig_t config = {};
+    config.gridDim            = dim3(1);
+    config.blockDim           = dim3(64);
+    config.stream             = static_cast<cudaStream_t>(stream);
+    cudaError_t e = cudaLaunchKernelEx(&config, spmm_b200::linear_wait_that_runs_out_kernel, static_cast<uint64_t>(limit_ms) * 1000000ull);
+    if (e != cudaSuccess)
+        (void)cudaGetLastError();
+    return static_cast<int>(e);
 }
 
 int spmm_b200_linear_plan(int tiles, int kb, int workers, int overhead, int pieces, int worker, int index, int* segment)

@@ -284,7 +284,9 @@ cudaError_t launch(cudaStream_t stream, void (*kern)(P...), dim3 grid, Args... a
     config.attrs                                       = attr;
     config.numAttrs                                    = 1;
     cudaError_t e = cudaLaunchKernelEx(&config, kern, args...);
-    return e != cudaSuccess ? e : cudaGetLastError();
+    if (e != cudaSuccess)
+        (void)cudaGetLastError();
+    return e;  // not what an earlier call has left behind
 }
 
 }  // namespace

@@ -589,3 +589,29 @@ def test_a_wait_that_runs_out_is_reported_and_cleared(sp):
     assert sp.device_status() == 0
     for n in (20, 300):
         run_case(sp, 1, 264, n, 528, None, torch.float16, None, True, integer_operands, True)
+
+
+def test_errors_of_other_calls_are_not_reported(sp):
+    """An error that an earlier call has returned already (here: the status is asked for while a stream is capturing) is not
+    returned again by a product or a quantiser that runs."""
+    import ctypes
+    runtime = ctypes.CDLL("libcudart.so.12")
+    m, n, k = 128, 4, 128
+    a, sa, b, sb, av, bv = random_operands(1, m, n, k, None, 1)
+    x = torch.ones((n, k), dtype=torch.float16, device="cuda")
+    c = torch.full((n, m), 7.0, dtype=torch.float16, device="cuda")
+    assert sp.fp8_linear(None, a, sa, b, sb, c, m, n, k, None) == 0 and sp.device_status() == 0
+    calls = [lambda: sp.quantize_fp8(None, x, b, sb, 1), lambda: sp.fp8_linear(None, a, sa, b, sb, c, m, n, k, None)]
+    for run in calls:
+        stream, graph = torch.cuda.Stream(), ctypes.c_void_p()
+        torch.cuda.synchronize()
+        assert runtime.cudaStreamBeginCapture(ctypes.c_void_p(stream.cuda_stream), 2) == 0
+        try:
+            status = sp.device_status()
+        finally:
+            runtime.cudaStreamEndCapture(ctypes.c_void_p(stream.cuda_stream), ctypes.byref(graph))
+            runtime.cudaGetLastError()
+        assert status < 0
+        assert run() == 0
+    assert sp.device_status() == 0
+    assert bool((b.float() == 448).all()) and bool((sb == 1 / torch.tensor(448.0, device="cuda")).all())
