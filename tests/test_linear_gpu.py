@@ -615,3 +615,91 @@ def test_errors_of_other_calls_are_not_reported(sp):
         assert run() == 0
     assert sp.device_status() == 0
     assert bool((b.float() == 448).all()) and bool((sb == 1 / torch.tensor(448.0, device="cuda")).all())
+
+
+# ---------------------------------------------------------------- scales, depth, many groups and bands of tiles
+def scaled_integer_operands(groups, m, n, k, dtype, seed):
+    """As integer_operands (A has about 40 places that are not zero in a row, whatever K is), but with scales drawn per block
+    and per token: 1 or 2 for A; 1/2, 1 or 2 for B.  Sums are multiples of 1/2 that stay below 128, exact in bf16, and a
+    scale of another k-block, row block, group or token, or a k-block left out, changes them at every depth."""
+    a, sa, b, sb, av, bv = integer_operands(groups, m, n, k, dtype, seed)
+    if dtype is not None:
+        return a, sa, b, sb, av, bv
+    g = rng(groups, m, n, k, seed, 2)
+    sa = torch.randint(0, 2, sa.shape, device="cuda", generator=g).float().exp2()
+    sb = torch.randint(-1, 2, sb.shape, device="cuda", generator=g).float().exp2()
+    av = a.double() * sa.double().repeat_interleave(128, 1)[:, :m].repeat_interleave(128, 2)[:, :, :k]
+    bv = b.double() * sb.double().t().repeat_interleave(128, 1)[:, :k]
+    return a, sa, b, sb, av, bv
+
+
+def exact_case(sp, groups, m, n, k, dtype, out, offsets, with_workspace):
+    """run_case on scaled_integer_operands, after a look at the oracle: its values have to fit the type of C."""
+    _, _, _, _, av, bv = scaled_integer_operands(groups, m, n, k, dtype, 5)
+    for e in range(groups):
+        want = bv[:256] @ av[e].t()
+        assert torch.equal(want.to(out).double(), want)
+    run_case(sp, groups, m, n, k, dtype, out, offsets, with_workspace, scaled_integer_operands, True)
+
+
+@pytest.mark.parametrize("with_workspace", [True, False], ids=["workspace", "alone"])
+@pytest.mark.parametrize("out", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("m,n,k", DENSE + [(264, 150, 16400), (520, 33, 9232), (640, 520, 4112)])
+def test_fp8_linear_with_scales_of_their_own(sp, m, n, k, out, with_workspace):
+    exact_case(sp, 1, m, n, k, None, out, None, with_workspace)
+
+
+@pytest.mark.parametrize("out", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+@pytest.mark.parametrize("case", range(len(GROUPED)))
+def test_grouped_fp8_with_scales_of_their_own(sp, case, out):
+    m, n, k, sizes, start = GROUPED[case]
+    exact_case(sp, len(sizes), m, n, k, None, out, borders(sizes, start), True)
+
+
+DEEP = [(128, 3, 36864), (2304, 16, 9216), (1000, 64, 8192), (264, 120, 16400), (640, 513, 8192)]
+
+
+@pytest.mark.parametrize("kind", ["e4m3-fp16", "e4m3-bf16", "fp16", "bf16"])
+@pytest.mark.parametrize("m,n,k", DEEP)
+def test_deep_products_by_their_mean_square_error(sp, m, n, k, kind):
+    """At large K the bound for each element, which adds up the largest error of every addition, hides whole k-blocks.  Of the
+    root of the mean square the triangle inequality gives more: an addition is off by 2^-23 of the sum there is at most,
+    K of them by K * 2^-23 times the largest root mean square that the sums have on their way (taken behind each 128; half as
+    much again for what lies between), and C by half a step.  A k-block left out is sqrt(128 / K) of C, more than five times that."""
+    out = torch.bfloat16 if kind.endswith("bf16") else torch.float16
+    dtype = None if kind.startswith("e4m3") else out
+    a, sa, b, sb, av, bv = random_operands(1, m, n, k, dtype, 7)
+    rms = lambda t: t.square().mean().sqrt().item()  # noqa: E731
+    total, largest = torch.zeros((n, m), dtype=torch.float64, device="cuda"), 0.0
+    for first in range(0, k, 128):
+        total += bv[:, first:first + 128] @ av[0][:, first:first + 128].t()
+        largest = max(largest, rms(total))
+    bound = HALF_STEP[out] * rms(total) + k * 2.0 ** -23 * 1.5 * largest
+    assert 5 * bound < (128.0 / k) ** 0.5 * rms(total)
+    off = None if dtype is None else torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    for ws in (None, workspace_for(sp, 1, m, n, k, dtype is None)):
+        c = torch.full((n, m), 7.0, dtype=out, device="cuda")
+        assert call(sp, a, sa, b, sb, c, off, 1, m, n, k, ws) == 0
+        assert rms(c.double() - total) <= bound
+
+
+@pytest.mark.parametrize("kind", ["fp16", "bf16", "e4m3-fp16", "e4m3-bf16"])
+def test_many_groups_of_many_tokens(sp, kind):
+    """More groups than are sorted by width (256), with 130 tokens on average: pairs of SMs."""
+    out = torch.bfloat16 if kind.endswith("bf16") else torch.float16
+    groups, m, k = 300, 264, 144
+    sizes = np.random.RandomState(3).multinomial(groups * 130, np.random.RandomState(4).dirichlet(np.full(groups, 0.7)))
+    sizes[17] = sizes[299] = 0
+    n = int(sizes.sum()) + 9
+    assert n // groups > 128 and (sizes > 512).any() and (sizes[:256] == 0).any()
+    run_case(sp, groups, m, n, k, None if kind.startswith("e4m3") else out, out, borders(sizes, 4), True, scaled_integer_operands, True)
+
+
+@pytest.mark.parametrize("kind", ["fp16", "bf16", "e4m3-fp16", "e4m3-bf16"])
+def test_several_bands_of_tiles(sp, kind):
+    """More tiles of tokens than a band holds (8), on pairs of SMs and in single blocks; every row is compared."""
+    out = torch.bfloat16 if kind.endswith("bf16") else torch.float16
+    dtype = None if kind.startswith("e4m3") else out
+    run_case(sp, 2, 776, 6300, 272, dtype, out, [3, 6221, 6290], True, scaled_integer_operands, True)
+    sizes = [0] * 20 + [4900] + [0] * 30
+    run_case(sp, len(sizes), 520, 4907, 272, dtype, out, borders(sizes, 7), True, scaled_integer_operands, True)
