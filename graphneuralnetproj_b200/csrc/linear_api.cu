@@ -32,9 +32,9 @@ bool aligned16(const void* p)
     return (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
 }
 
-// Which kernel, and tokens per tile.  One block per tile takes 128 tokens at most: one matrix is cut into as few tiles of
-// equal width as that allows; groups, whose sizes the host does not know, into tiles of twice the average, so that most
-// groups are one tile and its ring stages are not mostly unused.
+// Which kernel, and tokens per tile.  One block per tile takes 128 tokens at most.  All tokens of one matrix fit a tile then
+// (there would be pairs with more of them); the tokens of groups, whose sizes the host does not know, are cut into tiles of
+// twice the average, so that most groups are one tile and its ring stages are not mostly unused.
 void choose_tiles(LinearShape& s)
 {
     s.kb            = (s.k * (s.eight ? 1 : 2) - 1) / 128 + 1;
@@ -47,9 +47,8 @@ void choose_tiles(LinearShape& s)
         return;
     }
     if (!s.ragged) {
-        const int tiles = std::max(1, (s.n - 1) / 128 + 1);
-        s.nt            = std::max(16, ((s.n - 1) / tiles + 1 + 15) / 16 * 16);
-        s.b_box         = s.nt;
+        s.nt    = (s.n + 15) / 16 * 16;
+        s.b_box = s.nt;
     }
     else {
         const long want = std::min<long>(s.n, 2L * s.n / s.groups);

@@ -287,7 +287,6 @@ class _Torch:
         cls.single = (torch.float32,)
         cls.index = (torch.int32,)
         cls.current_device = torch.cuda.current_device
-        cls.current_stream = torch.cuda.current_stream
         # the handle alone, without a Stream object around it, where this torch has it
         cls.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
         cls.ready = True
