@@ -63,17 +63,25 @@ int max_workers(const LinearShape& s)
     return s.pair ? kMaxWorkers / 2 : kMaxWorkers;
 }
 
-// When cutting tiles pays (linear_plan.h), from measurements.  Few tokens: a block streams a step (32 KB) in 0.43 us, cutting costs
-// 4 us up to 32 tokens (1 token, 4096 x 4096, 32 tiles of 16 steps: 11.5 us whole, 10.6 in three parts; 9216 x 9216, 72 of 36: 20.7
-// and 21.4 where memory answers fast, 39 and 30 where it does not, and twice the blocks have twice the loads on their way), 7 us
-// up to 64 (64 x 2048 x 4096: 13.9 and 15.5).  Over 64 tokens a step takes as long as its arithmetic, about 1 us (90 x 4096 x
-// 2048, 32 tiles of 8: 12.1 and 15.3; 100 x 7168 x 7168, 56 of 28: 38 and 24.6).  Pairs: a piece is 128 KB per block, a k-block
-// 0.5 us (512 x 4096 x 14336, 32 tiles of 112: 60 us whole, 43 in two parts; 200 x 2048 x 2048, 8 of 16: 14.8 and 19.1).
+// What cutting a tile costs (linear_plan.h), in steps (k-blocks of pairs), from measurements of whole and cut tiles.  It depends
+// on the width: a step of 16 bits has half the features, and no additions on its way.  Times in us, weights m x k.
+//   up to 32 tokens     8 bits  16 x 2048 x 4096 (16 steps): 11.4 whole, 10.2 cut;  16 x 4096 x 2048 (8): 8.2 and 9.3
+//                      16 bits  16 x 4096 x 4096 (32): 16.2 and 12.3;  16 x 4096 x 2048 (16): 10.0 and 9.5
+//   up to 64            8 bits  33 x 7168 x 7168 (28): 20.0 and 18.2;  64 x 2048 x 4096 (16): 13.4 and 12.3;  64 x 4096 x 2048 (8): 9.5 and 11.2
+//                      16 bits  64 x 7168 x 7168 (56): 28.4 and 25.9;  61 x 320 x 2880 (23): 13.8 and 11.1;  33 x 4096 x 2048 (16): 11.2 and 11.6
+//   up to 128           8 bits  100 x 7168 x 7168 (28): 29.8 and 23.7;  128 x 4096 x 4096 (16): 20.0 and 18.4;  128 x 4096 x 2048 (8): 12.5 and 14.6
+//                      16 bits  100 x 7168 x 7168 (56): 32.3 and 29.8;  2 x 2640 x 4304 with 137 (34): 23.9 and 21.4;  128 x 4096 x 2048 (16): 12.0 and 15.2
+//   pairs               8 bits  200 x 7168 x 7168 (56): 32.5 and 28.4;  512 x 4096 x 4096 (32): 21.4 and 22.5
+//                      16 bits  200 x 1024 x 8192 (128): 38.2 and 30.5;  200 x 7168 x 7168 (112): 36.2 and 37.5;  200 x 4096 x 2048 (32): 15.5 and 27.3
 LinearCutting cutting(const LinearShape& s)
 {
     if (s.pair)
-        return LinearCutting{14, 4};
-    return LinearCutting{s.nt <= 32 ? 9 : (s.nt <= 64 ? 17 : 8), 16};
+        return LinearCutting{s.eight ? 18 : 62, 4};
+    if (s.nt <= 32)
+        return LinearCutting{9, 16};
+    if (s.nt <= 64)
+        return LinearCutting{s.eight ? 9 : 12, 16};
+    return LinearCutting{s.eight ? 8 : 20, 16};
 }
 
 size_t workspace_needed(const LinearShape& s)

@@ -703,3 +703,21 @@ def test_several_bands_of_tiles(sp, kind):
     run_case(sp, 2, 776, 6300, 272, dtype, out, [3, 6221, 6290], True, scaled_integer_operands, True)
     sizes = [0] * 20 + [4900] + [0] * 30
     run_case(sp, len(sizes), 520, 4907, 272, dtype, out, borders(sizes, 7), True, scaled_integer_operands, True)
+
+
+@pytest.mark.parametrize("kind,n,m,k,cut", [
+    ("bf16", 16, 4096, 4096, True), ("bf16", 64, 7168, 7168, True), ("bf16", 33, 4096, 2048, False), ("bf16", 100, 7168, 7168, True),
+    ("bf16", 128, 4096, 2048, False), ("bf16", 200, 1024, 8192, True), ("bf16", 200, 4096, 2048, False), ("bf16", 200, 7168, 7168, False),
+    ("e4m3", 16, 2048, 4096, True), ("e4m3", 16, 4096, 2048, False), ("e4m3", 33, 7168, 7168, True), ("e4m3", 64, 4096, 2048, False),
+    ("e4m3", 128, 4096, 4096, True), ("e4m3", 128, 4096, 2048, False), ("e4m3", 200, 7168, 7168, True), ("e4m3", 512, 4096, 4096, False)])
+def test_tiles_are_cut_where_that_is_faster(sp, kind, n, m, k, cut):
+    """Sizes at which whole and cut tiles were timed on a B200: pieces are parked in the workspace where cutting won, for each
+    width of the operands, and it stays as it is where whole tiles did.  The results are the same up to the order of sums."""
+    dtype = None if kind == "e4m3" else torch.bfloat16
+    a, sa, b, sb, av, bv = scaled_integer_operands(1, m, n, k, dtype, 5)
+    off = None if dtype is None else torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    c = torch.full((n, m), 7.0, dtype=torch.bfloat16, device="cuda")
+    ws = workspace_for(sp, 1, m, n, k, dtype is None)
+    assert call(sp, a, sa, b, sb, c, off, 1, m, n, k, ws) == 0
+    check(c, av, bv, None, k, torch.bfloat16, True)
+    assert bool(ws.any()) == cut
