@@ -328,11 +328,12 @@ extern "C" int spmm_b200_allreduce_status(int reset)
 {
     int         status = 0;
     cudaError_t e      = cudaDeviceSynchronize();
-    if (e != cudaSuccess)
+    if (e == cudaSuccess)
+        e = cudaMemcpyFromSymbol(&status, spmm_b200::g_device_status_allreduce, sizeof(int));
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();  // do not leave the error behind for an unrelated later call
         return -static_cast<int>(e);
-    e = cudaMemcpyFromSymbol(&status, spmm_b200::g_device_status_allreduce, sizeof(int));
-    if (e != cudaSuccess)
-        return -static_cast<int>(e);
+    }
     if (reset) {
         const int zero = 0;
         cudaMemcpyToSymbol(spmm_b200::g_device_status_allreduce, &zero, sizeof(int));

@@ -969,11 +969,12 @@ int spmm_b200_device_status(int reset)
 {
     int         status = 0;
     cudaError_t e      = cudaDeviceSynchronize();
-    if (e != cudaSuccess)
+    if (e == cudaSuccess)
+        e = cudaMemcpyFromSymbol(&status, spmm_b200::g_device_status, sizeof(int));
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();  // do not leave the error behind for an unrelated later call
         return -static_cast<int>(e);
-    e = cudaMemcpyFromSymbol(&status, spmm_b200::g_device_status, sizeof(int));
-    if (e != cudaSuccess)
-        return -static_cast<int>(e);
+    }
     if (reset) {
         const int zero = 0;
         cudaMemcpyToSymbol(spmm_b200::g_device_status, &zero, sizeof(int));

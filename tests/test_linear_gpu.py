@@ -592,8 +592,8 @@ def test_a_wait_that_runs_out_is_reported_and_cleared(sp):
 
 
 def test_errors_of_other_calls_are_not_reported(sp):
-    """An error that an earlier call has returned already (here: the status is asked for while a stream is capturing) is not
-    returned again by a product or a quantiser that runs."""
+    """An error that an earlier call has returned already (here: a status is asked for while a stream is capturing) is not
+    returned again by a product, a quantiser or an SpMM that runs."""
     import ctypes
     runtime = ctypes.CDLL("libcudart.so.12")
     m, n, k = 128, 4, 128
@@ -601,13 +601,18 @@ def test_errors_of_other_calls_are_not_reported(sp):
     x = torch.ones((n, k), dtype=torch.float16, device="cuda")
     c = torch.full((n, m), 7.0, dtype=torch.float16, device="cuda")
     assert sp.fp8_linear(None, a, sa, b, sb, c, m, n, k, None) == 0 and sp.device_status() == 0
-    calls = [lambda: sp.quantize_fp8(None, x, b, sb, 1), lambda: sp.fp8_linear(None, a, sa, b, sb, c, m, n, k, None)]
-    for run in calls:
+    words, offsets, _ = sp.InitSparseMatrixA_API(sp.synth_fp16((m, k), 1, 0.02, 0.8), m, 16, k)
+    words, offsets = torch.from_numpy(words.view(np.int32)).cuda(), torch.from_numpy(offsets).cuda()
+    dense, out = torch.ones((k, 16), dtype=torch.float16, device="cuda"), torch.empty((m, 16), dtype=torch.float16, device="cuda")
+    calls = [lambda: sp.quantize_fp8(None, x, b, sb, 1), lambda: sp.fp8_linear(None, a, sa, b, sb, c, m, n, k, None),
+             lambda: sp.SpMM_SplitK_API(None, None, words, None, None, offsets, dense, out, m, 16, k, None, 1)]
+    statuses = [sp.device_status, lambda: sp.spmm_api.LIB.spmm_b200_allreduce_status(0)]
+    for run, ask in [(run, ask) for run in calls for ask in statuses]:
         stream, graph = torch.cuda.Stream(), ctypes.c_void_p()
         torch.cuda.synchronize()
         assert runtime.cudaStreamBeginCapture(ctypes.c_void_p(stream.cuda_stream), 2) == 0
         try:
-            status = sp.device_status()
+            status = ask()
         finally:
             runtime.cudaStreamEndCapture(ctypes.c_void_p(stream.cuda_stream), ctypes.byref(graph))
             runtime.cudaGetLastError()
