@@ -13,9 +13,9 @@
 // columns); with tokens as columns each column needs its own factor out of shared memory, which costs as much of shared
 // memory's time as the operands do.
 //
-// What bounds them.  16 bits: the tensor core (2048 x 9472 x 4096: 112 us against 97 at the measured cuBLAS rate, tensor pipe
-// active 78 %).  Codes: the way round a TMEM buffer -- MMA, commit, wake-up, read-out, additions, arrival at the leader, next MMA --
-// of which there are two.  A k-block takes 0.51 us, about 840 cycles (2048 x 9472 x 8192: 148 us, tensor pipe 48 %); 0.46 without
+// What bounds them.  16 bits: the tensor core (2048 x 9472 x 4096: 111 us against 97 at the measured cuBLAS rate, tensor pipe
+// active 83 %).  Codes: the way round a TMEM buffer -- MMA, commit, wake-up, read-out, additions, arrival at the leader, next MMA --
+// of which there are two.  A k-block takes 0.51 us, about 840 cycles (2048 x 9472 x 8192: 149 us, tensor pipe 52 %); 0.46 without
 // the TMA loads, 0.48 without the scales, 0.40 without both; the protocol by itself, on operands that stay in shared memory, takes
 // 600 cycles, without the additions the 512 of the MMA.  (Additions that never stall starve the MMA warp of their scheduler: 909
 // cycles; the reads out of TMEM between them prevent that.)  Measured and dropped: four warpgroups (9 % slower, bound by

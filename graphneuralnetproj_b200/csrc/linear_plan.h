@@ -10,7 +10,7 @@
 //
 // Equal parts, although (tiles * parts) workers may be fewer than there are: with runs of equal length over all workers, run
 // borders lie anywhere in a tile, tiles have more pieces and workers two of them (28 tiles of 56 k-blocks on 74 pairs: 37 us,
-// 31 with two parts each on 56 of them).
+// 31 with two parts each on 56 of them; 28 since stores have become wider).
 #pragma once
 
 #include <cstdint>

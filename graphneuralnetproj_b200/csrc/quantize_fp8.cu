@@ -219,7 +219,8 @@ quantize_rows_kernel(const uint4* __restrict__ x, uint4* __restrict__ codes, flo
 
 // Blocks of 128 x 128, one per thread block: 8 lanes per row, 32 rows per pass, the whole block (32 KB) in registers
 // between the one read and the one write.  Four of them per SM: with two (the registers the compiler would take) the loads of
-// one do not cover the arithmetic of the other (9208 x 36864: 247 us, 188 with four, 238 with five, which spills).
+// one do not cover the arithmetic of the other (9208 x 36864, in a graph: 233 us, 179 with three, 156 with four, 219 with five,
+// which spills).
 template<bool BF16>
 __global__ void __launch_bounds__(256, 4)
 quantize_blocks_kernel(const uint4* __restrict__ x, uint4* __restrict__ codes, float* __restrict__ scales, int rows, int cols, int kb,

@@ -354,8 +354,8 @@ def quantize_fp8(stream, X, codes, scales, block_rows):
 
 
 def linear_workspace_bytes(groups, M_Global, N_Global, K_Global, eight_bit):
-    """Bytes of (once zero-filled) workspace for fp8_linear (groups = 1), grouped_linear and grouped_fp8_linear; 0 for sizes
-    that they refuse."""
+    """Bytes of workspace for fp8_linear (groups = 1), grouped_linear and grouped_fp8_linear; 0 for sizes that they refuse.  Fill it
+    with zeros once, and again after device_status() has reported that a wait gave up."""
     if (groups | M_Global | N_Global | K_Global) >> 31:
         return 0
     return int(LIB.spmm_b200_linear_workspace_bytes(groups, M_Global, N_Global, K_Global, int(eight_bit)))

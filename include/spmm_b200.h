@@ -328,7 +328,8 @@ void spmm_b200_decompose_v1(const uint16_t* A, uint16_t* A1, uint16_t* A2, int l
  *   weights      one scale per 128 x 128 block:            A_scales[groups][ceil(M / 128)][KB]
  *   activations  one per token and 128 features of it:     B_scales[KB][N]  (tokens contiguous)
  * A value is code * scale.  Products of codes are summed in fp32 by the tensor core over 128 features, times
- * the two scales, and summed in fp32 over the KB blocks; C is rounded once.
+ * the two scales, and summed in fp32 over the KB blocks; C is rounded once.  (The two scales are multiplied first, so their
+ * product has to be an fp32 number as well; the ones that the quantiser gives for values up to 2^70 always have one.)
  *
  * All calls are asynchronous on `stream`, allocate nothing and may be captured in a CUDA graph (make the first
  * call on a device outside a capture, as for the SpMM).  A, B, codes and workspaces start on 16-byte boundaries.

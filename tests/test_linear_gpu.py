@@ -499,6 +499,8 @@ def test_as_many_tokens_as_there_may_be(sp, eight):
     for first in range(2, n - 1, 1 << 26):
         last = min(n - 1, first + (1 << 26))
         assert torch.equal(c[first:last, 0], b[first:last].to(torch.float16).sum(1)), first
+    del a, b, c, sa, sb
+    torch.cuda.empty_cache()
 
 
 @pytest.mark.parametrize("kb", [1, 3, 4, 7], ids=lambda kb: "%d-blocks" % kb)
