@@ -728,3 +728,26 @@ def test_tiles_are_cut_where_that_is_faster(sp, kind, n, m, k, cut):
     assert call(sp, a, sa, b, sb, c, off, 1, m, n, k, ws) == 0
     check(c, av, bv, None, k, torch.bfloat16, True)
     assert bool(ws.any()) == cut
+
+
+@pytest.mark.parametrize("eight", [True, False], ids=["e4m3", "fp16"])
+def test_as_many_features_as_an_int_holds(sp, eight):
+    """2^31 - 8 rows of A of the smallest depth, one token: the same values and sums as with as many tokens."""
+    m, n, k = 2 ** 31 - 8, 1, 16 if eight else 8
+    free = torch.cuda.mem_get_info()[0]
+    if free < 64 << 30:
+        pytest.skip("needs 64 GB of device memory, %d GB are free" % (free >> 30))
+    a = torch.randint(0, 3 if eight else 2, (m, k), dtype=torch.uint8 if eight else torch.int16, device="cuda", generator=rng(m, k))
+    a.mul_(0x38 if eight else 0x3c00)
+    a = a.view(torch.float8_e4m3fn if eight else torch.float16)
+    b = torch.ones((n, k), device="cuda").to(a.dtype)
+    c = torch.full((n, m), 7.0, dtype=torch.float16, device="cuda")
+    off = None if eight else torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    sa, sb = (torch.ones((kb_of(m), 1), device="cuda"), torch.ones((1, n), device="cuda")) if eight else (None, None)
+    assert call(sp, a, sa, b, sb, c, off, 1, m, n, k, workspace_for(sp, 1, m, n, k, eight)) == 0
+    assert sp.device_status() == 0
+    for first in range(0, m, 1 << 26):
+        rows = slice(first, min(m, first + (1 << 26)))
+        assert torch.equal(c[0, rows], a[rows].to(torch.float16).sum(1)), first
+    del a, b, c, sa, sb
+    torch.cuda.empty_cache()
