@@ -70,7 +70,7 @@ int max_workers(const LinearShape& s)
 //   up to 64            8 bits  33 x 7168 x 7168 (28): 20.0 and 18.2;  64 x 2048 x 4096 (16): 13.4 and 12.3;  64 x 4096 x 2048 (8): 9.5 and 11.2
 //                      16 bits  64 x 7168 x 7168 (56): 28.4 and 25.9;  61 x 320 x 2880 (23): 13.8 and 11.1;  33 x 4096 x 2048 (16): 11.2 and 11.6
 //   up to 128           8 bits  100 x 7168 x 7168 (28): 29.8 and 23.7;  128 x 4096 x 4096 (16): 20.0 and 18.4;  128 x 4096 x 2048 (8): 12.5 and 14.6
-//                      16 bits  100 x 7168 x 7168 (56): 32.3 and 29.8;  2 x 2640 x 4304 with 137 (34): 23.9 and 21.4;  128 x 4096 x 2048 (16): 12.0 and 15.2
+//                      16 bits  100 x 7168 x 7168 (56): 32.3 and 29.8;  137 over 2 x 2640 x 4304 (34): 23.9 and 21.4;  128 x 4096 x 2048 (16): 12.0 and 15.2
 //   pairs               8 bits  200 x 7168 x 7168 (56): 32.5 and 28.4;  512 x 4096 x 4096 (32): 21.4 and 22.5
 //                      16 bits  200 x 1024 x 8192 (128): 38.2 and 30.5;  200 x 7168 x 7168 (112): 36.2 and 37.5;  200 x 4096 x 2048 (32): 15.5 and 27.3
 LinearCutting cutting(const LinearShape& s)

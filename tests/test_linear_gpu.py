@@ -751,3 +751,32 @@ def test_as_many_features_as_an_int_holds(sp, eight):
         assert torch.equal(c[0, rows], a[rows].to(torch.float16).sum(1)), first
     del a, b, c, sa, sb
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("with_workspace", [True, False], ids=["workspace", "alone"])
+@pytest.mark.parametrize("kind,n", [("bf16", 1), ("bf16", 129), ("e4m3", 1)])
+def test_as_deep_as_there_may_be(sp, kind, n, with_workspace):
+    """The largest K: one accumulation of 2^27 in 16 bits ends before a wait gives up, on one SM and on a pair.  Ones in 64
+    places of A, the first and the last among them, and one of 0, 1, -1 in each place of B: sums are exact."""
+    eight = kind == "e4m3"
+    m, k, dtype = 2, 2 ** 29 if eight else 2 ** 27, torch.float8_e4m3fn if eight else torch.bfloat16
+    free = torch.cuda.mem_get_info()[0]
+    if free < 48 << 30:
+        pytest.skip("needs 48 GB of device memory, %d GB are free" % (free >> 30))
+    places = torch.randint(0, k, (62,), device="cuda", generator=rng(k, n)).cpu().tolist() + [0, k - 1]
+    one = 0x38 if eight else 0x3f80
+    minus = (0x38 | 0x80) if eight else 0x3f80 - 0x8000  # as the stored integer
+    bits = torch.uint8 if eight else torch.int16
+    a, b = torch.zeros((1, m, k), dtype=bits, device="cuda"), torch.zeros((n, k), dtype=bits, device="cuda")
+    a[0, 1, places] = one
+    b[:, ::3] = one
+    b[:, 1::3] = minus
+    a, b = a.view(dtype), b.view(dtype)
+    sa, sb = (torch.ones((1, 1, kb_of(k)), device="cuda"), torch.ones((kb_of(k), n), device="cuda")) if eight else (None, None)
+    off = None if eight else torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    c = torch.full((n, m), 7.0, dtype=torch.bfloat16, device="cuda")
+    assert call(sp, a, sa, b, sb, c, off, 1, m, n, k, workspace_for(sp, 1, m, n, k, eight) if with_workspace else None) == 0
+    assert sp.device_status() == 0
+    assert bool((c[:, 0] == 0).all()) and bool((c[:, 1] == sum((1, -1, 0)[p % 3] for p in set(places))).all())
+    del a, b, c, sa, sb
+    torch.cuda.empty_cache()
